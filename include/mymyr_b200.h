@@ -414,6 +414,109 @@ b2_status b2_env_step_ex(b2_env* env, const b2_env_batch* batch, const b2_step_o
 b2_status b2_env_check_errors(b2_env* env);
 void b2_env_destroy(b2_env* env);
 
+/* ------------------------------------------------------------------------------------------------ learner
+ * Operators of a policy trained over the environments and expansions above: embedding lookup, log-probabilities of
+ * given tokens (actions) and the AdamW step. They have no counterpart in the reference. Every call is asynchronous on
+ * `stream`, allocates nothing and can be captured in a CUDA graph; device memory is the caller's. Calls on a context
+ * run on its device and leave the thread's current device as it was. */
+enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };
+
+enum { B2_TOP_MAX = 32 };
+
+/* Rows of logits: dense, row r at logits + r * row_stride, `width` long; or ragged (offsets set), row r at
+ * [offsets[r], offsets[r + 1]) of a vector of `width` logits (the CSR of b2_expand), rows bounded by it whatever the
+ * offsets say. A masked token, or one with logit -inf, has no probability. */
+typedef struct b2_logprobs_args {
+    const void* logits;
+    int32_t dtype;           /* B2_F32, B2_BF16 or B2_F16 */
+    int32_t offsets_bits;    /* 32 or 64 (int32_t or int64_t) */
+    uint64_t rows;
+    uint64_t width;          /* below 2^32 */
+    uint64_t row_stride;     /* dense rows, in elements (0: the same row for all) */
+    const void* offsets;     /* [rows + 1]; NULL: dense */
+    const void* tokens;      /* [rows] within the row; negative: no token. NULL: no tokens at all */
+    int32_t token_bits;      /* 32 or 64 */
+    uint32_t top;            /* alternatives, at most B2_TOP_MAX */
+    const uint8_t* mask;     /* nonzero: allowed. Dense: rows of `width` bytes, mask_stride apart; ragged: [width] */
+    uint64_t mask_stride;
+    float temperature;       /* > 0, finite: logits are divided by it */
+    float* logprob;          /* [rows]; required with tokens */
+    float* entropy;          /* [rows] */
+    float* stats;            /* [rows, 4], 16-byte aligned, or NULL: what the backward pass needs of a row (its largest
+                                logit, the log of its sum of exp((x - largest) / T), its entropy, unused) */
+    float* top_logprobs;     /* [rows, top], from the best down; -inf past the row's tokens */
+    int64_t* top_tokens;     /* [rows, top]; equal logits in index order; -1 past the row's tokens */
+} b2_logprobs_args;
+
+/* Log-probability of each row's token under softmax(logits / temperature), the row's entropy and its `top` most
+ * probable tokens. A row that leaves nothing (empty, all masked, all -inf): log-probabilities -inf, entropy 0, no
+ * alternatives. A token the mask excludes: -inf; a negative token: 0; a token past the row: NaN. NaN or +inf among a
+ * row's allowed logits: all of its values NaN, no alternatives. */
+b2_status b2_logprobs(b2_ctx* ctx, const b2_logprobs_args* args, void* stream);
+
+/* The gradient of the logits from those of logprob and entropy (either may be NULL), given the call's arguments with
+ * the stats that it wrote. grad_logits: same type as the logits, dense rows grad_stride apart, or ragged
+ * [width] (elements outside every row are not written). Zero for masked tokens and rows that leave nothing. */
+b2_status b2_logprobs_backward(b2_ctx* ctx, const b2_logprobs_args* args, const float* grad_logprob,
+                               const float* grad_entropy, void* grad_logits, uint64_t grad_stride, void* stream);
+
+typedef struct b2_embedding_args {
+    const void* tokens;      /* [count] */
+    int32_t token_bits;      /* 32 or 64 */
+    int32_t dtype;           /* of weight, rows, grad and grad_weight */
+    uint64_t count;          /* below 2^31 */
+    uint64_t vocabulary;     /* below 2^31 */
+    uint64_t width;
+    float scale;
+} b2_embedding_args;
+
+/* rows[i] = scale * weight[tokens[i]]; weight rows are weight_stride elements apart, `rows` is dense. A negative token
+ * gives a row of zeros, one past the vocabulary a row of NaN. */
+b2_status b2_embedding(b2_ctx* ctx, const b2_embedding_args* args, const void* weight, uint64_t weight_stride,
+                       void* rows, void* stream);
+
+/* grad_weight[v] = scale * (the sum of grad[i] over the places i with tokens[i] = v, in 32 bits and in the same order
+ * on every call), for every v of the vocabulary (grad_weight is dense, written whole); grad rows are grad_stride
+ * elements apart. Tokens outside the vocabulary add nothing. `workspace` holds b2_embedding_workspace() bytes, 16-byte
+ * aligned, of any contents. */
+size_t b2_embedding_workspace(const b2_embedding_args* args);
+b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, const void* grad, uint64_t grad_stride,
+                                void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+enum { B2_MOMENT_BLOCK = 256 };
+
+/* A tensor of an AdamW step: `elements` contiguous parameters and gradients, their moments from block `block` on
+ * (element block * B2_MOMENT_BLOCK of the moment arrays; tensors do not share blocks). */
+typedef struct b2_adamw_tensor {
+    void* param;
+    const void* grad;
+    uint64_t elements;
+    uint32_t block;
+    uint32_t reserved;
+} b2_adamw_tensor;
+
+typedef struct b2_adamw_args {
+    const b2_adamw_tensor* tensors; /* host memory, read during the call */
+    uint32_t count;
+    int32_t param_dtype;     /* B2_F32, B2_BF16 or B2_F16 */
+    int32_t grad_dtype;      /* param_dtype or B2_F32 */
+    int32_t moment_bits;     /* 32: float moments; 8: float8 e4m3 codes with a scale for each block */
+    uint64_t blocks;         /* of the moment arrays */
+    void* exp_avg;           /* [blocks * 256] */
+    void* exp_avg_sq;        /* [blocks * 256]; 8 bits: the codes of the second moment's square root */
+    float* exp_avg_scale;    /* [blocks], 8 bits */
+    float* exp_avg_sq_scale; /* [blocks], 8 bits */
+    float* master;           /* [blocks * 256] 32-bit parameters the 16-bit ones are rounded from, or NULL */
+    double lr, beta1, beta2, eps, weight_decay;
+    uint64_t step;           /* of this update, from 1 */
+    uint32_t seed;           /* 8 bits: of the second moment's rounding */
+} b2_adamw_args;
+
+/* m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2; p = p (1 - lr weight_decay) - lr m' / (sqrt(v') + eps)
+ * with m' = m / (1 - beta1^step), v' = v / (1 - beta2^step), in 32 bits, for every tensor: one launch for up to 96
+ * tensors or each 1,000 of them. */
+b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

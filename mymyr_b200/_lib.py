@@ -136,6 +136,37 @@ class StepOut(C.Structure):
                 ("binding", C.c_void_p), ("label_width", C.c_uint32), ("invalid", C.c_void_p), ("goal", C.c_void_p)]
 
 
+B2_TOP_MAX = 32
+B2_MOMENT_BLOCK = 256
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("offsets_bits", C.c_int32), ("rows", C.c_uint64),
+                ("width", C.c_uint64), ("row_stride", C.c_uint64), ("offsets", C.c_void_p), ("tokens", C.c_void_p),
+                ("token_bits", C.c_int32), ("top", C.c_uint32), ("mask", C.c_void_p), ("mask_stride", C.c_uint64),
+                ("temperature", C.c_float), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("top_tokens", C.c_void_p)]
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("token_bits", C.c_int32), ("dtype", C.c_int32), ("count", C.c_uint64),
+                ("vocabulary", C.c_uint64), ("width", C.c_uint64), ("scale", C.c_float)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("elements", C.c_uint64), ("block", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [("tensors", C.c_void_p), ("count", C.c_uint32), ("param_dtype", C.c_int32),
+                ("grad_dtype", C.c_int32), ("moment_bits", C.c_int32), ("blocks", C.c_uint64),
+                ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p),
+                ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("step", C.c_uint64),
+                ("seed", C.c_uint32)]
+
+
 P = C.c_void_p
 PP = C.POINTER(C.c_void_p)
 U32, U64, I32 = C.c_uint32, C.c_uint64, C.c_int32
@@ -188,6 +219,12 @@ SIGNATURES = {
     "b2_env_step_ex": (C.c_int, [P, C.POINTER(EnvBatch), C.POINTER(StepOut), P, P, P]),
     "b2_env_check_errors": (C.c_int, [P]),
     "b2_env_destroy": (None, [P]),
+    "b2_logprobs": (C.c_int, [P, C.POINTER(LogprobsArgs), P]),
+    "b2_logprobs_backward": (C.c_int, [P, C.POINTER(LogprobsArgs), P, P, P, U64, P]),
+    "b2_embedding": (C.c_int, [P, C.POINTER(EmbeddingArgs), P, U64, P, P]),
+    "b2_embedding_workspace": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
+    "b2_embedding_backward": (C.c_int, [P, C.POINTER(EmbeddingArgs), P, U64, P, P, C.c_size_t, P]),
+    "b2_adamw": (C.c_int, [P, C.POINTER(AdamwArgs), P]),
 }
 
 _lib = None
