@@ -55,131 +55,290 @@ __host__ __device__ __forceinline__ u32 mix(u32 x)
     return x;
 }
 
-__device__ __forceinline__ float e4m3_to_f32(u32 code)
+/// Two 32-bit numbers in a register pair, for the packed arithmetic of sm_100 (each half rounds as the plain operation).
+struct Two
 {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3);
-    return __half2float(h);
+    u64 v;
+    Two() = default;
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float2 get() const
+    {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b)
+{
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b)
+{
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
 }
 
-__device__ __forceinline__ u32 f32_to_e4m3(float x)
+/// Eight consecutive elements: one 32-byte or 16-byte access.
+__device__ __forceinline__ void load8(const float* p, float (&x)[8])
 {
-    // the conversion saturates infinities; they are no moments, so they become NaN as NaN does
-    return fabsf(x) < __builtin_huge_valf() ? __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3) : 0x7Fu;
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8])
+{
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                 "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+}
+template<class T>
+struct alignas(16) Eight
+{
+    T v[8];
+};
+template<class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8])
+{
+    const Eight<T> e = *reinterpret_cast<const Eight<T>*>(p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        x[k] = to_f32(e.v[k]);
+}
+template<class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8])
+{
+    Eight<T> e;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        e.v[k] = from_f32<T>(x[k]);
+    *reinterpret_cast<Eight<T>*>(p) = e;
+}
+template<class T>
+constexpr uintptr_t kAlign8 = sizeof(T) * 8 - 1;
+
+/// Eight e4m3 codes as 32-bit numbers, and back (NaN stays NaN; infinities saturate).
+__device__ __forceinline__ void decode8(uint2 c, float (&x)[8])
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+    {
+        const u32 word = k < 2 ? c.x : c.y;
+        const auto pair = static_cast<__nv_fp8x2_storage_t>(word >> (k & 1 ? 16 : 0));
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(pair, __NV_E4M3)));
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint2 encode8(const float (&x)[8])
+{
+    u32 h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        h[k] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+    return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-/// The power of two that brings the warp's largest finite magnitude to [128, 256).
-__device__ __forceinline__ float block_scale(u32 largest)
+__device__ __forceinline__ float sqrt_approx(float x)
 {
-    largest = __reduce_max_sync(~0u, largest);
-    const u32 e = largest & 0x7F800000u;
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+constexpr u32 kInfBits = 0x7F800000u;
+
+/// The power of two that brings a finite magnitude to [128, 256).
+__device__ __forceinline__ float scale_of(u32 largest)
+{
+    const u32 e = largest & kInfBits;
     return __uint_as_float(e > (8u << 23) ? e - (7u << 23) : 1u << 23);
 }
+/// 1 / scale, exactly.
+__device__ __forceinline__ float inverse_power(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
 
-__device__ __forceinline__ u32 finite_magnitude(float x)
+/// The warp's largest finite magnitude, as bits. Magnitudes order as their bits do; where an infinity or a NaN leads, the
+/// others are looked through again without it.
+__device__ __forceinline__ u32 largest_of(const float (&x)[8])
 {
-    const u32 u = __float_as_uint(x) & 0x7FFFFFFFu;
-    return u < 0x7F800000u ? u : 0u;
+    u32 top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+    u32 all = __reduce_max_sync(~0u, top);
+    if (all >= kInfBits)
+    {
+        top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+        {
+            const u32 u = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+            top = max(top, u < kInfBits ? u : 0u);
+        }
+        all = __reduce_max_sync(~0u, top) | 0x80000000u;  // the sign: some were left out
+    }
+    return all;
 }
 
-/// A warp for each block of 256 elements, lane l with elements l, l + 32, ...
+/// A warp for each block of 256 elements, lane l with the eight from 8 l on.
+///
+/// Bound by HBM in 32 bits (28 bytes for an element: parameter, gradient and moments read, all but the gradient written)
+/// and nearly as much by instruction issue in 8 bits (10 bytes). One pass: everything of an element is in registers
+/// between its loads and its stores, the block's largest magnitudes come from the warp's 32-bit maximum reduction, and
+/// the moments' arithmetic runs in pairs. Averages are separate multiplications and additions (not fused): the scales
+/// then are those of the formula as written, on any machine.
 template<class P, class G, int BITS, bool MASTER, u32 N>
 __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
                                                        u32 key)
 {
-    const u32 lane = threadIdx.x & 31;
-    for (u32 b = blockIdx.x * kWarps + (threadIdx.x >> 5); b < t.blocks; b += gridDim.x * kWarps)
+    const u32 lane = threadIdx.x & 31, i0 = lane * 8;
+    u32 b = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    u32 entry = 0;
     {
-        u32 lo = 0, hi = t.count;
-        while (hi - lo > 1)
+        u32 hi = t.count;
+        while (hi - entry > 1)
         {
-            const u32 mid = (lo + hi) / 2;
-            (t.e[mid].begin <= b ? lo : hi) = mid;
+            const u32 mid = (entry + hi) / 2;
+            (t.e[mid].begin <= b ? entry : hi) = mid;
         }
-        const Entry& e = t.e[lo];
+    }
+    for (; b < t.blocks; b += gridDim.x * kWarps)
+    {
+        while (entry + 1 < t.count && t.e[entry + 1].begin <= b)
+            ++entry;
+        const Entry& e = t.e[entry];
         const u64 first = static_cast<u64>(b - e.begin) * kMoment;  // in the tensor
         const u32 block = e.block + (b - e.begin);
-        const u64 at = static_cast<u64>(block) * kMoment;  // in the moments
+        const u64 at = static_cast<u64>(block) * kMoment + i0;  // in the moments, which hold whole blocks
         const u32 n = static_cast<u32>(e.n - first < kMoment ? e.n - first : kMoment);
-        P* p = static_cast<P*>(e.p) + first;
-        const G* g = static_cast<const G*>(e.g) + first;
-        float mk[8], rk[8];
-        u32 m_top = 0, r_top = 0;
-        float ms = 0, vs = 0;
+        P* const p = static_cast<P*>(e.p) + first + i0;
+        const G* const g = static_cast<const G*>(e.g) + first + i0;
+        // a tensor's last block, and tensors that start off a vector's boundary, go element by element
+        const bool whole = n == kMoment && !(reinterpret_cast<uintptr_t>(e.p) & kAlign8<P>) &&
+                           !(reinterpret_cast<uintptr_t>(e.g) & kAlign8<G>);
+        float gi[8], now[8], m[8], v[8], r[8];
+        if (whole)
+        {
+            load8(g, gi);
+            if (!MASTER)
+                load8(p, now);
+        }
+        else
+        {
+#pragma unroll
+            for (u32 k = 0; k < 8; ++k)
+            {
+                gi[k] = i0 + k < n ? to_f32(g[k]) : 0.f;
+                if (!MASTER)
+                    now[k] = i0 + k < n ? to_f32(p[k]) : 0.f;
+            }
+        }
+        if constexpr (MASTER)
+            load8(s.master + at, now);
         if constexpr (BITS == 8)
         {
-            ms = s.m_scale[block];
-            vs = s.v_scale[block];
+            decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.m) + at), m);
+            decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.v) + at), r);
+            const float ms = s.m_scale[block], vs = s.v_scale[block];
+            const Two ms2(ms, ms), vs2(vs, vs);
+#pragma unroll
+            for (int k = 0; k < 8; k += 2)
+            {
+                const float2 x = (Two(m[k], m[k + 1]) * ms2).get();
+                const Two y = Two(r[k], r[k + 1]) * vs2;
+                const float2 z = (y * y).get();
+                m[k] = x.x, m[k + 1] = x.y, v[k] = z.x, v[k + 1] = z.y;
+            }
+        }
+        else
+        {
+            load8(static_cast<const float*>(s.m) + at, m);
+            load8(static_cast<const float*>(s.v) + at, v);
+        }
+        const Two b1(h.b1, h.b1), a1(h.a1, h.a1), b2(h.b2, h.b2), a2(h.a2, h.a2);
+#pragma unroll
+        for (int k = 0; k < 8; k += 2)
+        {
+            const Two g2(gi[k], gi[k + 1]);
+            const float2 x = (Two(m[k], m[k + 1]) * b1 + g2 * a1).get();
+            const float2 y = (Two(v[k], v[k + 1]) * b2 + g2 * g2 * a2).get();
+            m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
         }
 #pragma unroll
-        for (u32 k = 0; k < 8; ++k)
+        for (int k = 0; k < 8; ++k)
         {
-            const u32 i = k * 32 + lane;
-            mk[k] = rk[k] = 0;
-            if (i >= n)
-                continue;
-            const float gi = to_f32(g[i]);
-            float m, v;
-            if constexpr (BITS == 8)
-            {
-                m = e4m3_to_f32(static_cast<const uint8_t*>(s.m)[at + i]) * ms;
-                const float r = e4m3_to_f32(static_cast<const uint8_t*>(s.v)[at + i]) * vs;
-                v = __fmul_rn(r, r);
-            }
-            else
-            {
-                m = static_cast<const float*>(s.m)[at + i];
-                v = static_cast<const float*>(s.v)[at + i];
-            }
-            m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gi, h.a1));
-            v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gi, gi), h.a2));
-            const float r = __fsqrt_rn(v);
-            const float old = MASTER ? s.master[at + i] : to_f32(p[i]);
-            const float now = old * h.decay - m / (r * h.correct + h.eps) * h.rate;
-            if (MASTER)
-                s.master[at + i] = now;
-            p[i] = from_f32<P>(now);
-            if constexpr (BITS == 32)
-            {
-                static_cast<float*>(s.m)[at + i] = m;
-                static_cast<float*>(s.v)[at + i] = v;
-            }
-            mk[k] = m;
-            rk[k] = r;
-            m_top = max(m_top, finite_magnitude(m));
-            r_top = max(r_top, finite_magnitude(r));
+            r[k] = sqrt_approx(v[k]);
+            now[k] = now[k] * h.decay - __fdividef(m[k] * h.rate, r[k] * h.correct + h.eps);
         }
-        if constexpr (BITS == 8)
+        if constexpr (MASTER)
+            store8(s.master + at, now);
+        if (whole)
+            store8(p, now);
+        else
         {
-            ms = block_scale(m_top);
-            vs = block_scale(r_top);
+#pragma unroll
+            for (u32 k = 0; k < 8; ++k)
+                if (i0 + k < n)
+                    p[k] = from_f32<P>(now[k]);
+        }
+        if constexpr (BITS == 32)
+        {
+            store8(static_cast<float*>(s.m) + at, m);
+            store8(static_cast<float*>(s.v) + at, v);
+        }
+        else
+        {
+            u32 top = largest_of(m);
+            bool bad = top >> 31;
+            const float ms = scale_of(top), mi = inverse_power(ms);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                m[k] *= mi;
+            if (bad)  // an infinity becomes NaN as NaN does, not the largest code
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    m[k] = m[k] - m[k] == 0.f ? m[k] : nanf("");
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + at) = encode8(m);
+            top = largest_of(v);
+            bad = top >> 31;
+            // the square root of the largest is the largest square root
+            const float vs = scale_of(__float_as_uint(__fsqrt_rn(__uint_as_float(top & 0x7FFFFFFFu))));
+            const float vi = inverse_power(vs);
+            float code[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += 2)
+            {
+                const u32 bits = mix((static_cast<u32>(at >> 1) + k / 2) ^ key);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                {
+                    // (16 bits + 1/2) / 2^16, by way of a number in [1, 2)
+                    const u32 part = j ? bits >> 16 : bits & 0xFFFFu;
+                    const float u = __uint_as_float(0x3F800040u | part << 7) - 1.f;
+                    // x / unit is in [8, 16), or below 8 among the smallest codes; its floor, by way of 2^23
+                    const float x = r[k + j] * vi;
+                    const u32 ex = max(__float_as_uint(x) & kInfBits, 121u << 23);
+                    const float q = x * __uint_as_float((257u << 23) - ex);
+                    const float low = __fadd_rd(q, 0x1p23f) - 0x1p23f;
+                    // up with the probability that keeps the square's mean: (q^2 - low^2) / ((low + 1)^2 - low^2)
+                    const float edge = fmaf(u, fmaf(2.f, low, 1.f), low * low);
+                    float c = (q * q > edge ? low + 1.f : low) * __uint_as_float(ex - (3u << 23));
+                    c = v[k + j] > 0.f ? fmaxf(c, 0x1p-9f) : 0.f;
+                    code[k + j] = c;
+                }
+            }
+            if (bad)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    code[k] = v[k] - v[k] == 0.f ? code[k] : nanf("");
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + at) = encode8(code);
             if (lane == 0)
             {
                 s.m_scale[block] = ms;
                 s.v_scale[block] = vs;
-            }
-#pragma unroll
-            for (u32 k = 0; k < 8; ++k)
-            {
-                const u32 i = k * 32 + lane;
-                if (i >= n)
-                    continue;
-                static_cast<uint8_t*>(s.m)[at + i] = static_cast<uint8_t>(f32_to_e4m3(mk[k] / ms));
-                const u64 el = at + i;
-                const u32 bits = mix(static_cast<u32>(el >> 1) ^ key);
-                const u32 k16 = el & 1 ? bits >> 16 : bits & 0xFFFFu;
-                const float u = (static_cast<float>(k16) + 0.5f) * 0x1p-16f;
-                float x = rk[k] / vs;
-                const u32 ex = max(__float_as_uint(x) & 0x7F800000u, 121u << 23);
-                const float unit = __uint_as_float(ex - (3u << 23));
-                x = x / unit;
-                const float low = floorf(x);
-                const float thr = __fadd_rn(__fmul_rn(low, low), __fmul_rn(u, 2 * low + 1));
-                float code = (low + (__fmul_rn(x, x) > thr ? 1.f : 0.f)) * unit;
-                if (code == 0.f && rk[k] > 0.f)
-                    code = 0x1p-9f;
-                if (!(rk[k] < __builtin_huge_valf()))
-                    code = nanf("");
-                static_cast<uint8_t*>(s.v)[at + i] = static_cast<uint8_t>(f32_to_e4m3(code));
             }
         }
     }
