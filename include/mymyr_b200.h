@@ -431,7 +431,7 @@ typedef struct b2_logprobs_args {
     int32_t dtype;           /* B2_F32, B2_BF16 or B2_F16 */
     int32_t offsets_bits;    /* 32 or 64 (int32_t or int64_t) */
     uint64_t rows;
-    uint64_t width;          /* below 2^32 */
+    uint64_t width;          /* below 2^32 - 256 */
     uint64_t row_stride;     /* dense rows, in elements (0: the same row for all) */
     const void* offsets;     /* [rows + 1]; NULL: dense */
     const void* tokens;      /* [rows] within the row; negative: no token. NULL: no tokens at all */

@@ -1,15 +1,32 @@
 // Log-probabilities of given tokens with entropy and the best alternatives, and the gradient of the logits.
 
+//
+// One pass over a row's logits x: with a reference r, S = sum 2^d and T = sum 2^d d for d = (x - r) log2(e) / temperature
+// give log-probabilities (x - r) / temperature - ln S and the entropy ln 2 (log2 S - T / S); partial sums of other
+// references join by shifting them. The best alternatives need no second pass over the row: a thread keeps the best of
+// the logits that it read, the k best threads hold the k best logits, and only their logits are read again (from cache).
+//
+// Bound by HBM where rows are long and many, by the latency of a few dependent steps where they are few, and by
+// instruction issue where they are short. So rows are laid out by their length: a group of 4, 8 or 32 lanes for a
+// short row, a block for a long one, a cluster of blocks (joined over distributed shared memory) where long rows are
+// too few to fill the device.
+
 #include "learn.cuh"
 
 #include <cmath>
+#include <cooperative_groups.h>
 
 namespace b2
 {
 namespace
 {
-constexpr int kBlock = 256;
+namespace cg = cooperative_groups;
+
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kAhead = 60.f;  // a sum's reference follows the row's maximum when it is this far ahead, in powers of two
 
 /// The rows of a call: row r's logits and mask, and its length, always inside the arrays.
 struct Rows
@@ -40,6 +57,7 @@ struct Rows
 struct Forward
 {
     Rows rows;
+    u64 count;
     const void* tokens;
     int token_bits;
     u32 top;
@@ -48,119 +66,13 @@ struct Forward
     long long* top_tokens;
 };
 
-/// Order of floats as unsigned integers; the two zeros are equal.
-__device__ __forceinline__ u32 ordered(float x)
-{
-    const u32 u = __float_as_uint(x + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ u64 block_max(u64 v, u64* tmp)
-{
-    for (int o = 16; o; o >>= 1)
-    {
-        const u64 w = __shfl_xor_sync(~0u, v, o);
-        v = w > v ? w : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0)
-        tmp[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = tmp[0];
-    for (int i = 1; i < kBlock / 32; ++i)
-        v = tmp[i] > v ? tmp[i] : v;
-    return v;
-}
-
-__device__ __forceinline__ float block_sum(float v, float* tmp)
-{
-    for (int o = 16; o; o >>= 1)
-        v += __shfl_xor_sync(~0u, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0)
-        tmp[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < kBlock / 32; ++i)
-        v += tmp[i];
-    return v;
-}
-
-template<class T>
-__global__ void __launch_bounds__(kBlock) k_logprobs(const Forward a)
-{
-    __shared__ u64 tmp[kBlock / 32];
-    __shared__ float ftmp[kBlock / 32];
-    const u64 r = blockIdx.x;
-    u64 begin, mbegin;
-    u32 len;
-    a.rows.at(r, begin, mbegin, len);
-    const T* x = static_cast<const T*>(a.rows.logits) + begin;
-    const uint8_t* mask = a.rows.mask ? a.rows.mask + mbegin : nullptr;
-    auto logit = [&](u32 j) { return mask && !mask[j] ? -kInf : to_f32(x[j]); };
-    // the largest logit by key (value, then lower index); NaN orders above +inf
-    u64 best = 0;
-    for (u32 j = threadIdx.x; j < len; j += kBlock)
-    {
-        const float v = logit(j);
-        const u64 k = static_cast<u64>(v != v ? ~0u : ordered(v)) << 32 | ~j;
-        best = k > best ? k : best;
-    }
-    best = block_max(best, tmp);
-    const float m = best ? logit(~static_cast<u32>(best)) : -kInf;
-    const bool dead = m == -kInf;
-    float s = 0, t = 0;
-    if (!dead)
-        for (u32 j = threadIdx.x; j < len; j += kBlock)
-        {
-            const float d = (logit(j) - m) * a.inv_t;
-            const float e = expf(d);
-            s += e;
-            t += e > 0 ? e * d : e;
-        }
-    s = block_sum(s, ftmp);
-    t = block_sum(t, ftmp);
-    const float logs = dead ? -kInf : logf(s);
-    const float h = dead ? 0.f : logs - t / s;
-    const bool bad = s != s;
-    auto logp = [&](float v) { return dead || v == -kInf ? (bad ? v - m + logs : -kInf) : (v - m) * a.inv_t - logs; };
-    if (threadIdx.x == 0)
-    {
-        if (a.tokens)
-        {
-            const long long y = token_at(a.tokens, a.token_bits, r);
-            a.logprob[r] = y < 0 ? 0.f : y >= len ? nanf("") : bad ? s : logp(logit(static_cast<u32>(y)));
-        }
-        a.entropy[r] = h;
-        if (a.stats)
-            reinterpret_cast<float4*>(a.stats)[r] = make_float4(m, logs, h, 0.f);
-    }
-    u64 last = best;
-    for (u32 i = 0; i < a.top; ++i)
-    {
-        const float v = last ? logit(~static_cast<u32>(last)) : -kInf;
-        if (threadIdx.x == 0)
-        {
-            const bool none = bad || v == -kInf;
-            a.top_tokens[r * a.top + i] = none ? -1 : static_cast<long long>(~static_cast<u32>(last));
-            a.top_logprobs[r * a.top + i] = bad ? s : none ? -kInf : logp(v);
-        }
-        u64 next = 0;
-        for (u32 j = threadIdx.x; j < len; j += kBlock)
-        {
-            const u64 k = static_cast<u64>(ordered(logit(j))) << 32 | ~j;
-            if (k < last)
-                next = k > next ? k : next;
-        }
-        last = block_max(next, tmp);
-    }
-}
-
 struct Backward
 {
     Rows rows;
+    u64 count;
     const void* tokens;
     int token_bits;
+    u32 slices;  // blocks of a long row
     float inv_t;
     const float* stats;
     const float *grad_logprob, *grad_entropy;
@@ -168,41 +80,648 @@ struct Backward
     u64 grad_stride;
 };
 
-template<class T>
-__global__ void __launch_bounds__(kBlock) k_logprobs_backward(const Backward a)
+__device__ __forceinline__ float exp2_approx(float x)
 {
-    const u64 r = blockIdx.x;
-    u64 begin, mbegin;
-    u32 len;
-    a.rows.at(r, begin, mbegin, len);
-    const T* x = static_cast<const T*>(a.rows.logits) + begin;
-    const uint8_t* mask = a.rows.mask ? a.rows.mask + mbegin : nullptr;
-    T* dx = static_cast<T*>(a.grad) + (a.rows.offsets ? begin : r * a.grad_stride);
-    const float4 st = reinterpret_cast<const float4*>(a.stats)[r];
-    const float m = st.x, logs = st.y, h = st.z;
-    const bool dead = m == -kInf;
-    float gl = a.grad_logprob ? a.grad_logprob[r] : 0.f;
-    const float ge = a.grad_entropy ? a.grad_entropy[r] : 0.f;
-    long long y = -1;
-    if (a.tokens && a.grad_logprob)
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+/// Order of floats as unsigned integers, and back; the two zeros are equal.
+__device__ __forceinline__ u32 ordered(float x)
+{
+    const u32 u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(u32 k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+/// A logit as a key: the larger logit, then the lower index, has the larger key; 0 stands for none.
+__device__ __forceinline__ u64 key_of(float x, u32 index)
+{
+    return x == -kInf ? 0 : static_cast<u64>(ordered(x)) << 32 | ~index;
+}
+__device__ __forceinline__ float logit_of(u64 key) { return key ? unordered(static_cast<u32>(key >> 32)) : -kInf; }
+__device__ __forceinline__ u32 index_of(u64 key) { return ~static_cast<u32>(key); }
+
+/// A row's sums about a reference: 2^d and 2^d d over its logits, and its largest logit.
+struct Sums
+{
+    float ref = kLowest, s = 0.f, t = 0.f, best = -kInf;
+
+    Sums() = default;
+    __device__ __forceinline__ explicit Sums(float4 v) : ref(v.x), s(v.y), t(v.z), best(v.w) {}
+    __device__ __forceinline__ float4 pack() const { return make_float4(ref, s, t, best); }
+    /// Moves the reference (up, or anywhere while the sums are empty).
+    __device__ __forceinline__ void move(float to, float c)
     {
-        y = token_at(a.tokens, a.token_bits, r);
-        gl = y < 0 ? 0.f : y >= len ? nanf("") : gl;
-    }
-    for (u32 j = threadIdx.x; j < len; j += kBlock)
-    {
-        float g = 0.f;
-        if (!dead && (!mask || mask[j]))
+        if (s != 0.f)
         {
-            const float v = to_f32(x[j]);
-            const float lp = (v - m) * a.inv_t - logs;
-            const float p = expf(lp);
-            g = -p * (gl + (p == 0.f ? 0.f : ge * (lp + h)));
-            if (j == y)
-                g += gl;
-            g *= a.inv_t;
+            const float d = (ref - to) * c, f = exp2_approx(d);
+            t = f > 0.f ? f * (t + s * d) : f;
+            s *= f;
         }
-        dx[j] = from_f32<T>(g);
+        ref = to;
+    }
+    /// Adds the sums of other logits; both come to stand about the larger of their largest.
+    __device__ __forceinline__ void join(Sums o, float c)
+    {
+        best = fmaxf(best, o.best);
+        if (best > -kInf)
+        {
+            move(best, c);
+            o.move(best, c);
+        }
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ void add(float x, float c)
+    {
+        const float d = (x - ref) * c, e = exp2_approx(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, -200.f), t);  // e is 0 there: minus infinity must not come in
+    }
+};
+
+/// The results of a row from its joined sums (s about ref): the same arithmetic on every path.
+struct Row
+{
+    float ref, log_s, entropy, inv_t;
+    bool dead, bad;
+    __device__ __forceinline__ Row(const Sums& a, float inv_temperature)
+        : ref(a.ref), inv_t(inv_temperature), dead(a.best == -kInf && a.s == a.s), bad(a.s != a.s)
+    {
+        const float l2 = __log2f(a.s);
+        log_s = dead ? -kInf : l2 * kLn2;
+        entropy = dead ? 0.f : (l2 - a.t / a.s) * kLn2;
+    }
+    __device__ __forceinline__ float logp(float x) const
+    {
+        return bad ? log_s : dead || x == -kInf ? -kInf : (x - ref) * inv_t - log_s;
+    }
+};
+
+__device__ __forceinline__ void store_row(const Forward& a, u64 r, const Row& row, long long token, u32 len, float logit)
+{
+    if (a.tokens)
+        a.logprob[r] = token < 0 ? 0.f : token >= len ? nanf("") : row.logp(logit);
+    a.entropy[r] = row.entropy;
+    if (a.stats)
+        reinterpret_cast<float4*>(a.stats)[r] = make_float4(row.dead ? -kInf : row.ref, row.log_s, row.entropy, 0.f);
+}
+
+__device__ __forceinline__ void store_top(const Forward& a, u64 r, u32 i, const Row& row, u64 key)
+{
+    const bool none = row.bad || !key;
+    a.top_tokens[r * a.top + i] = none ? -1 : static_cast<long long>(index_of(key));
+    a.top_logprobs[r * a.top + i] = row.logp(logit_of(key));
+}
+
+// ---------------------------------------------------------------------------------------------- sorted lists of a warp
+
+/// Lane i holds the i-th largest of 32 keys.
+__device__ __forceinline__ u64 exchange(u64 key, u32 with, bool larger)
+{
+    const u64 other = __shfl_xor_sync(~0u, key, with);
+    return (other > key) == larger ? other : key;
+}
+__device__ __forceinline__ u64 warp_sort(u64 key)
+{
+    const u32 lane = threadIdx.x & 31;
+#pragma unroll
+    for (u32 size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (u32 step = size / 2; step; step /= 2)
+            key = exchange(key, step, ((lane & step) == 0) == ((lane & size) == 0));
+    return key;
+}
+/// The 32 largest of two sorted lists, sorted; `reversed` is the other list from its smallest up.
+__device__ __forceinline__ u64 warp_merge(u64 key, u64 reversed)
+{
+    const u32 lane = threadIdx.x & 31;
+    key = reversed > key ? reversed : key;
+#pragma unroll
+    for (u32 step = 16; step; step /= 2)
+        key = exchange(key, step, (lane & step) == 0);
+    return key;
+}
+__device__ __forceinline__ u64 warp_insert(u64 list, u64 key)
+{
+    const u32 lane = threadIdx.x & 31;
+    const u32 at = __popc(__ballot_sync(~0u, list > key));
+    const u64 above = __shfl_up_sync(~0u, list, 1);
+    return lane < at ? list : lane == at ? key : above;
+}
+
+// ---------------------------------------------------------------------------------------------- short rows
+
+/// `G` lanes for a row (one warp at most); up to R logits in each lane's registers, longer rows by reading them again.
+template<class T, int G, int R>
+__global__ void __launch_bounds__(128) k_logprobs_short(const Forward a)
+{
+    const u32 lane = threadIdx.x & (G - 1);
+    const u64 r = (static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x) / G;
+    const bool live = r < a.count;
+    if (G == 32 && !live)
+        return;
+    u64 begin = 0, mask_begin = 0;
+    u32 len = 0;
+    long long token = -1;
+    if (live)
+    {
+        a.rows.at(r, begin, mask_begin, len);
+        if (a.tokens)
+            token = token_at(a.tokens, a.token_bits, r);
+    }
+    const T* x = static_cast<const T*>(a.rows.logits) + begin;
+    const uint8_t* mask = a.rows.mask ? a.rows.mask + mask_begin : nullptr;
+    auto logit = [&](u32 j) { return mask && !mask[j] ? -kInf : to_f32(x[j]); };
+    const float c = a.inv_t * kLog2e;
+    float v[R];
+    Sums sum;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+    {
+        const u32 j = i * G + lane;
+        v[i] = -kInf;
+        if (i * G < len)  // the same for the whole group
+            v[i] = j < len ? logit(j) : -kInf;
+        sum.best = fmaxf(sum.best, v[i]);
+    }
+    for (u32 j = R * G + lane; j < len; j += G)
+        sum.best = fmaxf(sum.best, logit(j));
+#pragma unroll
+    for (int o = G / 2; o; o /= 2)
+        sum.best = fmaxf(sum.best, __shfl_xor_sync(~0u, sum.best, o));
+    sum.ref = fmaxf(sum.best, kLowest);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (i * G < len)
+            sum.add(v[i], c);
+    for (u32 j = R * G + lane; j < len; j += G)
+        sum.add(logit(j), c);
+#pragma unroll
+    for (int o = G / 2; o; o /= 2)
+    {
+        sum.s += __shfl_xor_sync(~0u, sum.s, o);
+        sum.t += __shfl_xor_sync(~0u, sum.t, o);
+    }
+    const Row row(sum, a.inv_t);
+    if (live && lane == 0)
+        store_row(a, r, row, token, len, token >= 0 && token < len ? logit(static_cast<u32>(token)) : -kInf);
+    if (!a.top)
+        return;
+    if constexpr (G == 32)
+    {
+        u64 list = warp_sort(key_of(v[0], lane));
+        u64 least = __shfl_sync(~0u, list, a.top - 1);
+        auto offer = [&](u64 key) {
+            for (u32 more = __ballot_sync(~0u, key > least); more; more &= more - 1)
+            {
+                const u64 k = __shfl_sync(~0u, key, __ffs(more) - 1);
+                if (k > least)
+                {
+                    list = warp_insert(list, k);
+                    least = __shfl_sync(~0u, list, a.top - 1);
+                }
+            }
+        };
+#pragma unroll
+        for (int i = 1; i < R; ++i)
+            if (i * G < len)
+                offer(key_of(v[i], i * G + lane));
+        for (u32 j = R * G; j < len; j += G)
+            offer(j + lane < len ? key_of(logit(j + lane), j + lane) : 0);
+        if (lane < a.top)
+            store_top(a, r, lane, row, list);
+    }
+    else
+    {
+        u64 last = ~0ull;
+        for (u32 k = 0; k < a.top; ++k)
+        {
+            u64 best = 0;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+            {
+                const u64 key = key_of(v[i], i * G + lane);
+                if (key < last && key > best)
+                    best = key;
+            }
+            for (u32 j = R * G + lane; j < len; j += G)
+            {
+                const u64 key = key_of(logit(j), j);
+                if (key < last && key > best)
+                    best = key;
+            }
+#pragma unroll
+            for (int o = G / 2; o; o /= 2)
+            {
+                const u64 other = __shfl_xor_sync(~0u, best, o);
+                best = other > best ? other : best;
+            }
+            last = best;
+            if (live && lane == 0)
+                store_top(a, r, k, row, best);
+        }
+    }
+}
+
+/// One element of the gradient of the logits.
+struct Slope
+{
+    float ref, log_s, entropy, inv_t, gl, ge;
+    bool dead;
+    __device__ __forceinline__ Slope(const Backward& a, u64 r, long long& token, u32 len) : inv_t(a.inv_t)
+    {
+        const float4 st = reinterpret_cast<const float4*>(a.stats)[r];
+        ref = st.x, log_s = st.y, entropy = st.z;
+        dead = st.x == -kInf;
+        gl = a.grad_logprob ? a.grad_logprob[r] : 0.f;
+        ge = a.grad_entropy ? a.grad_entropy[r] : 0.f;
+        token = a.grad_logprob ? token_at(a.tokens, a.token_bits, r) : -1;
+        if (a.grad_logprob)
+            gl = token < 0 ? 0.f : token >= len ? nanf("") : gl;
+    }
+    __device__ __forceinline__ float operator()(float x, bool is_token) const
+    {
+        // below -200 the probability is 0: minus infinity must not come in
+        const float lp = fmaxf((x - ref) * inv_t - log_s, -200.f), p = exp2_approx(lp * kLog2e);
+        const float g = fmaf(-p, fmaf(ge, lp + entropy, gl), is_token ? gl : 0.f) * inv_t;
+        return log_s == log_s ? g : log_s;
+    }
+};
+
+template<class T, int G>
+__global__ void __launch_bounds__(128) k_logprobs_backward_short(const Backward a)
+{
+    const u32 lane = threadIdx.x & (G - 1);
+    const u64 r = (static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x) / G;
+    if (r >= a.count)
+        return;
+    u64 begin, mask_begin;
+    u32 len;
+    a.rows.at(r, begin, mask_begin, len);
+    const T* x = static_cast<const T*>(a.rows.logits) + begin;
+    const uint8_t* mask = a.rows.mask ? a.rows.mask + mask_begin : nullptr;
+    T* dx = static_cast<T*>(a.grad) + (a.rows.offsets ? begin : r * a.grad_stride);
+    long long token;
+    const Slope slope(a, r, token, len);
+#pragma unroll 4
+    for (u32 j = lane; j < len; j += G)
+        dx[j] = from_f32<T>(slope.dead || (mask && !mask[j]) ? 0.f : slope(to_f32(x[j]), j == token));
+}
+
+// ---------------------------------------------------------------------------------------------- long rows
+
+template<class T>
+constexpr int kVec = 16 / sizeof(T);
+
+/// A row as vectors of 16 aligned bytes; the first and the last may stick out of it.
+template<class T, bool MASK>
+struct Vectors
+{
+    static constexpr int VE = kVec<T>;
+    const T* base;        // of vector 0
+    const uint8_t* mask;  // of vector 0's first element
+    u32 shift, end, count;  // in elements of the vectors: the row is [shift, end)
+    bool mask_aligned;
+    __device__ __forceinline__ Vectors(const T* x, const uint8_t* m, u32 len)
+    {
+        shift = static_cast<u32>(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (VE - 1);
+        base = x - shift;
+        end = shift + len;
+        count = (static_cast<u64>(end) + VE - 1) / VE;
+        mask = MASK ? m - shift : nullptr;
+        mask_aligned = MASK && reinterpret_cast<uintptr_t>(mask) % VE == 0;
+    }
+    __device__ __forceinline__ bool whole(u32 i) const { return i * VE >= shift && end - i * VE >= VE; }
+    /// Vector i, -inf in masked places and outside of the row.
+    __device__ __forceinline__ void load_any(u32 i, float (&x)[VE]) const
+    {
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+        {
+            const u32 q = i * VE + k;
+            x[k] = q >= shift && q < end && (!MASK || mask[q]) ? to_f32(base[q]) : -kInf;
+        }
+    }
+    __device__ __forceinline__ uint4 load_raw(u32 i) const
+    {
+        return *reinterpret_cast<const uint4*>(base + static_cast<u64>(i) * VE);
+    }
+    __device__ __forceinline__ u64 load_mask(u32 i) const
+    {
+        if constexpr (!MASK)
+            return 0;
+        const uint8_t* m = mask + static_cast<u64>(i) * VE;
+        if (mask_aligned)
+            return VE == 8 ? *reinterpret_cast<const u64*>(m) : *reinterpret_cast<const u32*>(m);
+        u64 w = 0;
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+            w |= static_cast<u64>(m[k]) << (8 * k);
+        return w;
+    }
+    __device__ __forceinline__ static void unpack(uint4 raw, u64 allowed, float (&x)[VE])
+    {
+        struct alignas(16) E
+        {
+            T v[VE];
+        };
+        const E e = *reinterpret_cast<const E*>(&raw);
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+        {
+            x[k] = to_f32(e.v[k]);
+            if (MASK && !(allowed >> (8 * k) & 0xFF))
+                x[k] = -kInf;
+        }
+    }
+};
+
+template<int N>
+__device__ __forceinline__ float max_of(const float (&x)[N])
+{
+    float m = x[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k)
+        m = fmaxf(m, x[k]);
+    return m;
+}
+
+/// What a thread knows of the logits that it read: their sums, and the vector of the first of their largest.
+template<int VE>
+struct Scan
+{
+    Sums sum;
+    u32 at = 0;
+    __device__ __forceinline__ void add(const float (&x)[VE], u32 i, float c, float ahead)
+    {
+        const float m = max_of(x);
+        at = m > sum.best ? i : at;
+        sum.best = fmaxf(sum.best, m);
+        if (m > sum.ref + ahead)
+            sum.move(m, c);
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+            sum.add(x[k], c);
+    }
+};
+
+constexpr u32 kListKeys = 32;
+
+/// The 32 largest keys of a block's warps' sorted lists, in warp 0's lanes; `lists` holds 32 keys for each warp.
+template<int NW>
+__device__ __forceinline__ u64 block_merge(u64 list, u64* lists)
+{
+    const u32 lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int s = 1; s < NW; s *= 2)
+    {
+        if ((w & (2 * s - 1)) == s)
+            lists[w * kListKeys + lane] = list;
+        __syncthreads();
+        if ((w & (2 * s - 1)) == 0)
+            list = warp_merge(list, lists[(w + s) * kListKeys + 31 - lane]);
+    }
+    return list;
+}
+
+/// A block (of NW warps) for a row, or the C blocks of a cluster for a row, each with a run of its vectors.
+template<class T, bool MASK, int NW>
+__global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 cluster)
+{
+    constexpr int VE = kVec<T>, N = NW * 32, U = 4;
+    __shared__ u64 lists[NW * kListKeys];
+    __shared__ u64 threshold_keys[kListKeys];
+    __shared__ float4 sums[NW];  // of each warp
+    __shared__ float4 block_sums;
+    __shared__ u64 block_list[kListKeys];
+    const u32 tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const u64 r = blockIdx.x / cluster;
+    const u32 part = blockIdx.x % cluster;
+    u64 begin, mask_begin;
+    u32 len;
+    a.rows.at(r, begin, mask_begin, len);
+    const T* x = static_cast<const T*>(a.rows.logits) + begin;
+    const uint8_t* mask = MASK ? a.rows.mask + mask_begin : nullptr;
+    // the given token's logit, under way while the row is read
+    long long token = -1;
+    float given = -kInf;
+    if (tid == 0 && a.tokens)
+    {
+        token = token_at(a.tokens, a.token_bits, r);
+        if (token >= 0 && token < len && (!MASK || mask[token]))
+            given = to_f32(x[token]);
+    }
+    const Vectors<T, MASK> row(x, mask, len);
+    const u32 share = (row.count + cluster - 1) / cluster;
+    const u32 first = min(part * share, row.count), last = min(first + share, row.count);
+    const float c = a.inv_t * kLog2e, ahead = kAhead / c;
+    Scan<VE> scan;
+    u32 i = first + tid;
+    if (i < last && !row.whole(i))
+    {
+        float v[VE];
+        row.load_any(i, v);
+        scan.add(v, i, c, ahead);
+        i += N;
+    }
+    const u32 whole_end = last > first && !row.whole(last - 1) ? last - 1 : last;
+    for (; i + (U - 1) * N < whole_end; i += U * N)
+    {
+        uint4 raw[U];
+        u64 allowed[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+        {
+            raw[k] = row.load_raw(i + k * N);
+            allowed[k] = row.load_mask(i + k * N);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+        {
+            float v[VE];
+            row.unpack(raw[k], allowed[k], v);
+            scan.add(v, i + k * N, c, ahead);
+        }
+    }
+    for (; i < last; i += N)
+    {
+        float v[VE];
+        if (i < whole_end)
+            row.unpack(row.load_raw(i), row.load_mask(i), v);
+        else
+            row.load_any(i, v);
+        scan.add(v, i, c, ahead);
+    }
+    // the block's sums about its largest logit
+    Sums sum = scan.sum;
+    float best = sum.best;
+#pragma unroll
+    for (int o = 16; o; o /= 2)
+        best = fmaxf(best, __shfl_xor_sync(~0u, best, o));
+    if (best > -kInf)
+        sum.move(best, c);
+#pragma unroll
+    for (int o = 16; o; o /= 2)
+    {
+        sum.s += __shfl_xor_sync(~0u, sum.s, o);
+        sum.t += __shfl_xor_sync(~0u, sum.t, o);
+    }
+    sum.best = best;
+    if (lane == 0)
+        sums[w] = sum.pack();
+    u64 list = 0;
+    if (a.top)
+    {
+        // the threads' best; the top-th of them bounds what can be among the row's best
+        list = block_merge<NW>(warp_sort(key_of(scan.sum.best, scan.at)), lists);
+        if (w == 0)
+            threshold_keys[lane] = lane < a.top ? list : 0;
+    }
+    __syncthreads();
+    if (a.top)
+    {
+        list = 0;
+        const u64 bound = threshold_keys[a.top - 1];
+        for (u32 k = w; k < a.top && threshold_keys[k]; k += NW)
+        {
+            // the logits of the k-th best thread: every N-th vector
+            const u32 owner = (index_of(threshold_keys[k]) - first) % N;
+            for (u32 j0 = first + owner; j0 < last; j0 += 32 * N)
+            {
+                const u32 j = j0 + lane * N;
+                float v[VE];
+                bool any = false;
+                if (j < last && j >= j0)
+                {
+                    row.load_any(j, v);
+                    any = key_of(max_of(v), j) >= bound;
+                }
+                for (u32 more = __ballot_sync(~0u, any); more; more &= more - 1)
+                {
+                    const int src = __ffs(more) - 1;
+                    const u32 at = __shfl_sync(~0u, j, src) * VE - row.shift;
+#pragma unroll
+                    for (int q = 0; q < VE; ++q)
+                    {
+                        const float y = __shfl_sync(~0u, v[q], src);
+                        const u64 key = key_of(y, at + q);
+                        // warp-uniform: the list's last place is the bound for the rest
+                        if (key > __shfl_sync(~0u, list, 31))
+                            list = warp_insert(list, key);
+                    }
+                }
+            }
+        }
+        list = block_merge<NW>(list, lists);
+    }
+    if (w == 0)
+    {
+        sum = Sums(sums[0]);
+        for (int k = 1; k < NW; ++k)
+            sum.join(Sums(sums[k]), c);
+    }
+    if (cluster > 1)
+    {
+        cg::cluster_group group = cg::this_cluster();
+        if (w == 0)
+        {
+            if (lane == 0)
+                block_sums = sum.pack();
+            block_list[lane] = list;
+        }
+        group.sync();
+        if (part == 0 && w == 0)
+        {
+            for (u32 k = 1; k < cluster; ++k)
+            {
+                sum.join(Sums(*group.map_shared_rank(&block_sums, k)), c);
+                if (a.top)
+                    list = warp_merge(list, group.map_shared_rank(block_list, k)[31 - lane]);
+            }
+        }
+        group.sync();  // the other blocks' shared memory stays until it has been read
+    }
+    if (part == 0 && w == 0)
+    {
+        const Row out(sum, a.inv_t);
+        if (lane == 0)
+            store_row(a, r, out, token, len, given);
+        if (lane < a.top)
+            store_top(a, r, lane, out, list);
+    }
+}
+
+constexpr int kBackwardBlock = 256, kBackwardVectors = 4;
+
+template<class T, bool MASK>
+__global__ void __launch_bounds__(kBackwardBlock) k_logprobs_backward_long(const Backward a)
+{
+    constexpr int VE = kVec<T>, U = kBackwardVectors;
+    struct alignas(16) Out
+    {
+        T v[VE];
+    };
+    const u64 r = blockIdx.x / a.slices;
+    u64 begin, mask_begin;
+    u32 len;
+    a.rows.at(r, begin, mask_begin, len);
+    const Vectors<T, MASK> row(static_cast<const T*>(a.rows.logits) + begin,
+                               MASK ? a.rows.mask + mask_begin : nullptr, len);
+    T* const dx = static_cast<T*>(a.grad) + (a.rows.offsets ? begin : r * a.grad_stride) - row.shift;
+    const bool aligned = reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+    long long token;
+    const Slope slope(a, r, token, len);
+    const u32 token_at_vec = token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u;
+    for (u64 i0 = (blockIdx.x % a.slices) * static_cast<u64>(kBackwardBlock * U); i0 < row.count;
+         i0 += static_cast<u64>(a.slices) * kBackwardBlock * U)
+    {
+        const u32 i = static_cast<u32>(i0) + threadIdx.x;
+        uint4 raw[U];
+        u64 allowed[U];
+        bool whole[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+        {
+            const u32 j = i + k * kBackwardBlock;
+            whole[k] = j < row.count && row.whole(j);
+            if (whole[k])
+            {
+                raw[k] = row.load_raw(j);
+                allowed[k] = row.load_mask(j);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+        {
+            const u32 j = i + k * kBackwardBlock;
+            if (j >= row.count)
+                continue;
+            float v[VE];
+            if (whole[k])
+                row.unpack(raw[k], allowed[k], v);
+            else
+                row.load_any(j, v);
+            Out o;
+#pragma unroll
+            for (int q = 0; q < VE; ++q)
+            {
+                const float g = slope(v[q], j * VE + q == token_at_vec);
+                o.v[q] = from_f32<T>(slope.dead || (MASK && v[q] == -kInf) ? 0.f : g);
+            }
+            T* const to = dx + static_cast<u64>(j) * VE;
+            if (whole[k] && aligned)
+                *reinterpret_cast<Out*>(to) = o;
+            else
+            {
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    if (j * VE + q >= row.shift && j * VE + q < row.end)
+                        to[q] = o.v[q];
+            }
+        }
     }
 }
 
@@ -211,21 +730,95 @@ Rows rows_of(const b2_logprobs_args& a)
     return {a.logits, a.offsets, a.mask, a.row_stride, a.mask_stride, a.width, a.offsets_bits};
 }
 
+/// The mean length of a call's rows, by which they are laid out (ragged rows that are longer still are right, if slower).
+u64 mean_length(const Rows& rows, u64 count) { return rows.offsets ? rows.width / count : rows.width; }
+
+constexpr u64 kShort = 1024;
+
+template<class T, bool MASK, int NW>
+void forward_long(const Forward& f, u32 cluster, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(f.count) * cluster);
+    cfg.blockDim = dim3(NW * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    B2_CUDA(cudaLaunchKernelEx(&cfg, k_logprobs_long<T, MASK, NW>, f, cluster));
+}
+
+template<class T>
+void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
+{
+    const u64 mean = mean_length(f.rows, f.count);
+    if (mean <= kShort)
+    {
+        auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
+        if (mean <= 4)
+            k_logprobs_short<T, 4, 4><<<blocks(4), 128, 0, st>>>(f);
+        else if (mean <= 16)
+            k_logprobs_short<T, 8, 8><<<blocks(8), 128, 0, st>>>(f);
+        else
+            k_logprobs_short<T, 32, 32><<<blocks(32), 128, 0, st>>>(f);
+        return;
+    }
+    // blocks of 8 warps; a cluster for a row while its blocks still have two vectors for each thread and the device
+    // has room for all of them at twice a block for each SM
+    constexpr int NW = 8;
+    u32 cluster = 1;
+    while (cluster < 8 && f.count * cluster * 2 <= static_cast<u64>(ctx.sms) * 2 &&
+           mean >= static_cast<u64>(cluster) * 2 * NW * 32 * kVec<T> * 2)
+        cluster *= 2;
+    if (f.rows.mask)
+        forward_long<T, true, NW>(f, cluster, st);
+    else
+        forward_long<T, false, NW>(f, cluster, st);
+}
+
+template<class T>
+void backward(Backward f, cudaStream_t st)
+{
+    const u64 mean = mean_length(f.rows, f.count);
+    if (mean <= kShort)
+    {
+        auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
+        if (mean <= 4)
+            k_logprobs_backward_short<T, 4><<<blocks(4), 128, 0, st>>>(f);
+        else if (mean <= 16)
+            k_logprobs_backward_short<T, 8><<<blocks(8), 128, 0, st>>>(f);
+        else
+            k_logprobs_backward_short<T, 32><<<blocks(32), 128, 0, st>>>(f);
+        return;
+    }
+    constexpr u64 slice = static_cast<u64>(kBackwardBlock) * kBackwardVectors * kVec<T>;
+    const u64 most = ((1ull << 31) - 1) / f.count;
+    f.slices = static_cast<u32>(std::max<u64>(1, std::min<u64>((mean + slice - 1) / slice, most)));
+    const unsigned blocks = static_cast<unsigned>(f.count * f.slices);
+    if (f.rows.mask)
+        k_logprobs_backward_long<T, true><<<blocks, kBackwardBlock, 0, st>>>(f);
+    else
+        k_logprobs_backward_long<T, false><<<blocks, kBackwardBlock, 0, st>>>(f);
+}
+
 void check_args(b2_ctx* ctx, const b2_logprobs_args* a, const char* what)
 {
     auto bad = [&](const char* m) { return std::invalid_argument(std::string(what) + ": " + m); };
     if (!ctx || !a)
         throw bad("null argument");
-    if (a->rows >= 1ull << 31 || a->width >= 0xFFFFFFFFull)
-        throw bad("rows must be below 2^31 and width below 2^32 - 1");
+    if (a->rows >= 1ull << 31 || a->width >= 0xFFFFFF00ull)
+        throw bad("rows must be below 2^31 and width below 2^32 - 256");
     if (a->width && a->rows && !a->logits)
         throw bad("null logits");
     if (a->offsets && a->offsets_bits != 32 && a->offsets_bits != 64)
         throw bad("offsets must be of 32 or 64 bits");
     if (a->tokens && a->token_bits != 32 && a->token_bits != 64)
         throw bad("tokens must be of 32 or 64 bits");
-    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature))
-        throw bad("temperature must be positive and finite");
+    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.5f / a->temperature))
+        throw bad("temperature must be positive and finite, and its inverse too");
     if (a->top > B2_TOP_MAX)
         throw bad("more than 32 alternatives");
 }
@@ -247,9 +840,9 @@ b2_status b2_logprobs(b2_ctx* ctx, const b2_logprobs_args* args, void* stream)
             if (!a.rows)
                 return;
             const OnDevice on(ctx->device);
-            const Forward f{rows_of(a), a.tokens, a.token_bits, a.top, 1.f / a.temperature, a.logprob, a.entropy, a.stats,
+            const Forward f{rows_of(a), a.rows, a.tokens, a.token_bits, a.top, 1.f / a.temperature, a.logprob, a.entropy, a.stats,
                             a.top_logprobs, reinterpret_cast<long long*>(a.top_tokens)};
-            k_logprobs<T><<<static_cast<unsigned>(a.rows), kBlock, 0, static_cast<cudaStream_t>(stream)>>>(f);
+            forward<T>(*ctx, f, static_cast<cudaStream_t>(stream));
             B2_CUDA(cudaGetLastError());
         });
     });
@@ -267,10 +860,9 @@ b2_status b2_logprobs_backward(b2_ctx* ctx, const b2_logprobs_args* args, const 
             if (!a.rows || !a.width)
                 return;
             const OnDevice on(ctx->device);
-            const Backward f{rows_of(a), a.tokens, a.token_bits, 1.f / a.temperature, a.stats,
+            const Backward f{rows_of(a), a.rows, a.tokens, a.token_bits, 1, 1.f / a.temperature, a.stats,
                              a.tokens ? grad_logprob : nullptr, grad_entropy, grad_logits, grad_stride};
-            k_logprobs_backward<T>
-                <<<static_cast<unsigned>(a.rows), kBlock, 0, static_cast<cudaStream_t>(stream)>>>(f);
+            backward<T>(f, static_cast<cudaStream_t>(stream));
             B2_CUDA(cudaGetLastError());
         });
     });
