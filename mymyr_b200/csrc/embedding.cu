@@ -4,20 +4,23 @@
 // sorted by token with a stable radix sort, so that each token's places lie together in their own order; the sorted
 // list is cut into chunks of equal length, and one thread walks a chunk for one vector of columns, holding the running
 // sum in registers. A token that lies inside a chunk is written at once; one that crosses chunks leaves a partial sum
-// in each, which a last kernel adds in chunk order. No floating-point atomics: the same bits on every call.
+// in each, and a last kernel adds these in a fixed order. No floating-point atomics: the same bits on every call.
+//
+// Bound by HBM: each gradient row is read once and each row of the table's gradient written once, or twice where its
+// token occurs: the zeros go out while the sort, which needs a few SMs for some dependent steps, is under way.
 
 #include "learn.cuh"
+
+#include <cooperative_groups.h>
+#include <mutex>
 
 namespace b2
 {
 namespace
 {
-constexpr u32 kSortBlock = 256;
-constexpr u32 kSortRounds = 16;                            // 32 keys of a warp in each
-constexpr u32 kSortTile = kSortBlock * kSortRounds;        // keys of a block
-constexpr u32 kWarpKeys = 32 * kSortRounds;
-constexpr u32 kDigitBits = 8;
-constexpr u32 kBins = 1u << kDigitBits;
+namespace cg = cooperative_groups;
+
+constexpr u32 kBins = 256;  // digits have at most eight bits
 
 template<class T, int VE>
 struct alignas(sizeof(T) * VE) Vec
@@ -25,44 +28,74 @@ struct alignas(sizeof(T) * VE) Vec
     T v[VE];
 };
 
-/// Where a pass's keys come from: the tokens (a token outside the vocabulary sorts past the others), or the pass before.
-struct Keys
+/// The tokens as keys; one outside the vocabulary is no key.
+struct Tokens
 {
-    const void* tokens;  // first pass; null afterwards
-    const u32* keys;
-    const u32* places;
-    int token_bits;
+    const void* tokens;
+    int bits;
     u32 vocabulary;
-    __device__ __forceinline__ u32 key(u32 i) const
+    __device__ __forceinline__ bool key(u32 i, u32& k) const
     {
-        if (!tokens)
-            return keys[i];
-        const long long t = token_at(tokens, token_bits, i);
-        return t < 0 || t >= vocabulary ? vocabulary : static_cast<u32>(t);
+        const long long t = token_at(tokens, bits, i);
+        k = static_cast<u32>(t);
+        return t >= 0 && t < vocabulary;
     }
-    __device__ __forceinline__ u32 place(u32 i) const { return tokens ? i : places[i]; }
 };
 
-/// Counts of each digit in each tile: counts[digit * tiles + tile].
-__global__ void __launch_bounds__(kSortBlock) k_sort_count(const Keys in, u32 n, u32 shift, u32 tiles,
-                                                           u32* __restrict__ counts)
+/// Bytes to be set to zero by the blocks that a kernel has to spare.
+struct Zeros
 {
-    __shared__ u32 bins[kBins];
-    bins[threadIdx.x] = 0;
-    __syncthreads();
-    const u32 base = blockIdx.x * kSortTile;
-    for (u32 k = 0; k < kSortRounds; ++k)
-    {
-        const u32 i = base + k * kSortBlock + threadIdx.x;
-        if (i < n)
-            atomicAdd(&bins[in.key(i) >> shift & (kBins - 1)], 1u);
-    }
-    __syncthreads();
-    counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
+    void* p;
+    u64 bytes;
+};
+__device__ __forceinline__ void write_zeros(const Zeros& z, u64 thread, u64 threads)
+{
+    const u64 head = min(z.bytes, static_cast<u64>(-reinterpret_cast<uintptr_t>(z.p) & 15));
+    char* const p = static_cast<char*>(z.p);
+    uint4* const v = reinterpret_cast<uint4*>(p + head);
+    const u64 n = (z.bytes - head) / 16;
+    for (u64 i = thread; i < n; i += threads)
+        v[i] = make_uint4(0, 0, 0, 0);
+    const u64 tail = head + n * 16;
+    if (thread < head)
+        p[thread] = 0;
+    if (tail + thread < z.bytes && thread < 16)
+        p[tail + thread] = 0;
 }
 
-/// Exclusive sum over a block's 256 threads; *total the sum of all.
-__device__ __forceinline__ u32 block_exclusive(u32 v, u32* tmp, u32* total)
+/// The lanes of a warp that hold the same digit (of eight bits; the flag joins as a ninth).
+__device__ __forceinline__ u32 same_digit(u32 digit, bool held, u32 bits)
+{
+    u32 same = __ballot_sync(~0u, held);
+    same = held ? same : ~same;
+    for (u32 b = 0; b < bits; ++b)
+    {
+        const bool one = digit >> b & 1;
+        const u32 ones = __ballot_sync(~0u, one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+
+/// A key's rank among its warp's keys of the same digit so far; counts[digit] goes up by the warp's keys.
+__device__ __forceinline__ u32 warp_rank(u32 digit, bool held, u32 bits, u32* counts)
+{
+    const u32 lane = threadIdx.x & 31;
+    const u32 same = same_digit(digit, held, bits);
+    const u32 before = __popc(same & ((1u << lane) - 1));
+    u32 first = 0;
+    if (held && before == 0)
+    {
+        first = counts[digit];
+        counts[digit] = first + __popc(same);
+    }
+    __syncwarp();
+    return __shfl_sync(~0u, first, __ffs(same) - 1) + before;
+}
+
+/// Exclusive sum over a block's first 256 threads, which hold the digits' counts; *total the sum of all. Every thread
+/// of the block comes here.
+__device__ __forceinline__ u32 digits_exclusive(u32 v, u32* tmp, u32* total)
 {
     const u32 lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     u32 s = v;
@@ -73,11 +106,11 @@ __device__ __forceinline__ u32 block_exclusive(u32 v, u32* tmp, u32* total)
         s += lane >= o ? x : 0;
     }
     __syncthreads();
-    if (lane == 31)
+    if (lane == 31 && w < kBins / 32)
         tmp[w] = s;
     __syncthreads();
     u32 before = 0, all = 0;
-    for (u32 i = 0; i < kSortBlock / 32; ++i)
+    for (u32 i = 0; i < kBins / 32; ++i)
     {
         before += i < w ? tmp[i] : 0;
         all += tmp[i];
@@ -86,10 +119,187 @@ __device__ __forceinline__ u32 block_exclusive(u32 v, u32* tmp, u32* total)
     return before + s - v;
 }
 
+// ---------------------------------------------------------------------------------------------- sort in one cluster
+
+constexpr u32 kClusterBlocks = 8, kClusterThreads = 1024, kClusterWarps = 32;
+constexpr u32 kClusterRounds = 8;                                                      // keys of a thread
+constexpr u32 kClusterMost = kClusterBlocks * kClusterThreads * kClusterRounds;        // 65,536 keys
+
+/// The shared memory of a block: two sets of keys and places, the warps' counts of each digit, and their sums.
+constexpr size_t cluster_bytes(u32 share)
+{
+    return (static_cast<size_t>(share) * 4 + kClusterWarps * kBins + 2 * kBins + kBins / 32) * 4;
+}
+
+/// The first cluster sorts the keys, `share` in each block, handing them from block to block over distributed shared
+/// memory in each pass; the others write zeros. 16,383 tokens of 65,536 (two passes): 11 us, under the 134 MB of zeros
+/// of a table of 1,024 columns; as separate launches of count, scan and scatter kernels it took 44 us before them.
+__global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const Tokens in, u32 n, u32 share, u32 passes, u32 bits,
+                                                                  u32* __restrict__ keys, u32* __restrict__ places,
+                                                                  u32* __restrict__ held_count, const Zeros zeros)
+{
+    const u32 t = threadIdx.x, lane = t & 31, w = t >> 5;
+    if (blockIdx.x >= kClusterBlocks)
+    {
+        write_zeros(zeros, static_cast<u64>(blockIdx.x - kClusterBlocks) * kClusterThreads + t,
+                    static_cast<u64>(gridDim.x - kClusterBlocks) * kClusterThreads);
+        return;
+    }
+    extern __shared__ u32 shared[];
+    u32* const buffers = shared;  // [2][keys, places][share]
+    u32* const counts = shared + share * 4;
+    u32* const sums = counts + kClusterWarps * kBins;
+    u32* const base = sums + kBins;
+    u32* const tmp = base + kBins;
+    cg::cluster_group cluster = cg::this_cluster();
+    const u32 q = cluster.block_rank(), rounds = share / kClusterThreads;
+    const u32 local = w * (share / kClusterWarps) + lane;
+    u32 total = n;
+    for (u32 pass = 0; pass < passes; ++pass)
+    {
+        const u32 shift = pass * bits;
+        const u32* const from = buffers + (pass & 1) * 2 * share;
+        u32 key[kClusterRounds], place[kClusterRounds], rank[kClusterRounds], held = 0;
+        for (u32 i = t; i < kClusterWarps * kBins; i += kClusterThreads)
+            counts[i] = 0;
+#pragma unroll
+        for (u32 k = 0; k < kClusterRounds; ++k)
+        {
+            if (k >= rounds)
+                break;
+            const u32 j = local + k * 32, i = q * share + j;
+            key[k] = place[k] = 0;
+            bool is = i < total;
+            if (pass == 0)
+            {
+                is = is && in.key(i, key[k]);
+                place[k] = i;
+            }
+            else if (is)
+            {
+                key[k] = from[j];
+                place[k] = from[share + j];
+            }
+            held |= static_cast<u32>(is) << k;
+        }
+        __syncthreads();
+#pragma unroll
+        for (u32 k = 0; k < kClusterRounds; ++k)
+        {
+            if (k >= rounds)
+                break;
+            rank[k] = warp_rank(key[k] >> shift & ((1u << bits) - 1), held >> k & 1, bits, counts + w * kBins);
+        }
+        __syncthreads();
+        if (t < kBins)
+        {
+            u32 run = 0;
+            for (u32 i = 0; i < kClusterWarps; ++i)
+            {
+                const u32 c = counts[i * kBins + t];
+                counts[i * kBins + t] = run;
+                run += c;
+            }
+            sums[t] = run;
+        }
+        cluster.sync();
+        u32 all = 0, before = 0;
+        if (t < kBins)
+            for (u32 i = 0; i < kClusterBlocks; ++i)
+            {
+                const u32 c = cluster.map_shared_rank(sums, i)[t];
+                all += c;
+                before += i < q ? c : 0;
+            }
+        const u32 lower = digits_exclusive(all, tmp, &total);
+        if (t < kBins)
+            base[t] = lower + before;
+        __syncthreads();
+#pragma unroll
+        for (u32 k = 0; k < kClusterRounds; ++k)
+        {
+            if (k >= rounds)
+                break;
+            if (!(held >> k & 1))
+                continue;
+            const u32 digit = key[k] >> shift & ((1u << bits) - 1);
+            const u32 to = base[digit] + counts[w * kBins + digit] + rank[k];
+            if (pass + 1 == passes)
+            {
+                keys[to] = key[k];
+                places[to] = place[k];
+            }
+            else
+            {
+                u32* const b = cluster.map_shared_rank(buffers, to / share) + ((pass + 1) & 1) * 2 * share + to % share;
+                b[0] = key[k];
+                b[share] = place[k];
+            }
+        }
+        cluster.sync();
+    }
+    if (q == 0 && t == 0)
+        *held_count = total;
+}
+
+// ---------------------------------------------------------------------------------------------- sort over the device
+
+constexpr u32 kSortBlock = 256;
+constexpr u32 kSortRounds = 4;                       // 32 keys of a warp in each
+constexpr u32 kSortTile = kSortBlock * kSortRounds;  // keys of a block
+constexpr u32 kWarpKeys = 32 * kSortRounds;
+
+/// A pass's input: the tokens in the first, the pass before afterwards.
+struct Pass
+{
+    Tokens tokens;
+    const u32* keys;  // null in the first pass
+    const u32* places;
+    const u32* count;  // of the keys that are held; null in the first pass: n
+    u32 n, shift, bits, tiles;
+    __device__ __forceinline__ u32 size() const { return count ? *count : n; }
+    __device__ __forceinline__ bool key(u32 i, u32 size, u32& k) const
+    {
+        k = 0;
+        if (i >= size)
+            return false;
+        if (!keys)
+            return tokens.key(i, k);
+        k = keys[i];
+        return true;
+    }
+    __device__ __forceinline__ u32 place(u32 i) const { return keys ? places[i] : i; }
+    __device__ __forceinline__ u32 digit(u32 k) const { return k >> shift & ((1u << bits) - 1); }
+};
+
+/// Counts of each digit in each tile: counts[digit * tiles + tile]. Blocks past the tiles write zeros.
+__global__ void __launch_bounds__(kSortBlock) k_sort_count(const Pass in, u32* __restrict__ counts, const Zeros zeros)
+{
+    if (blockIdx.x >= in.tiles)
+    {
+        write_zeros(zeros, static_cast<u64>(blockIdx.x - in.tiles) * kSortBlock + threadIdx.x,
+                    static_cast<u64>(gridDim.x - in.tiles) * kSortBlock);
+        return;
+    }
+    __shared__ u32 bins[kBins];
+    bins[threadIdx.x] = 0;
+    __syncthreads();
+    const u32 base = blockIdx.x * kSortTile, size = in.size();
+#pragma unroll
+    for (u32 k = 0; k < kSortRounds; ++k)
+    {
+        u32 key;
+        if (in.key(base + k * kSortBlock + threadIdx.x, size, key))
+            atomicAdd(&bins[in.digit(key)], 1u);
+    }
+    __syncthreads();
+    counts[threadIdx.x * in.tiles + blockIdx.x] = bins[threadIdx.x];
+}
+
 /// A block for each digit: its tiles' counts become their exclusive sums, its total goes to totals[digit].
 __global__ void __launch_bounds__(kSortBlock) k_sort_scan(u32* __restrict__ counts, u32 tiles, u32* __restrict__ totals)
 {
-    __shared__ u32 tmp[kSortBlock / 32];
+    __shared__ u32 tmp[kBins / 32];
     u32* row = counts + static_cast<u64>(blockIdx.x) * tiles;
     u32 carry = 0;
     for (u32 t = 0; t < tiles; t += kSortBlock)
@@ -97,7 +307,7 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scan(u32* __restrict__ coun
         const u32 i = t + threadIdx.x;
         const u32 v = i < tiles ? row[i] : 0;
         u32 total;
-        const u32 e = block_exclusive(v, tmp, &total);
+        const u32 e = digits_exclusive(v, tmp, &total);
         if (i < tiles)
             row[i] = carry + e;
         carry += total;
@@ -106,70 +316,61 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scan(u32* __restrict__ coun
         totals[blockIdx.x] = carry;
 }
 
-/// Each key to its digit's place, equal digits in the order they came in.
-__global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Keys in, u32 n, u32 shift, u32 tiles,
-                                                             const u32* __restrict__ counts,
+/// Each key to its digit's place, equal digits in the order they came in; the number of keys to held_count.
+__global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Pass in, const u32* __restrict__ counts,
                                                              const u32* __restrict__ totals, u32* __restrict__ keys,
-                                                             u32* __restrict__ places)
+                                                             u32* __restrict__ places, u32* __restrict__ held_count)
 {
     __shared__ u32 at[kSortBlock / 32][kBins];
-    __shared__ u32 tmp[kSortBlock / 32];
+    __shared__ u32 tmp[kBins / 32];
     const u32 lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (u32 i = threadIdx.x; i < kBins * (kSortBlock / 32); i += kSortBlock)
         (&at[0][0])[i] = 0;
-    __syncthreads();
-    const u32 base = blockIdx.x * kSortTile + w * kWarpKeys;
-    u32 key[kSortRounds], rank[kSortRounds];
+    const u32 base = blockIdx.x * kSortTile + w * kWarpKeys, size = in.size();
+    u32 key[kSortRounds], place[kSortRounds], rank[kSortRounds], held = 0;
 #pragma unroll
     for (u32 k = 0; k < kSortRounds; ++k)
     {
         const u32 i = base + k * 32 + lane;
-        key[k] = i < n ? in.key(i) : 0;
-        const u32 digit = i < n ? key[k] >> shift & (kBins - 1) : kBins;  // absent keys: a digit of their own
-        const u32 same = __match_any_sync(~0u, digit);
-        const u32 before = __popc(same & ((1u << lane) - 1));
-        u32 first = 0;
-        if (i < n && before == 0)
-        {
-            first = at[w][digit];
-            at[w][digit] = first + __popc(same);
-        }
-        __syncwarp();
-        rank[k] = __shfl_sync(~0u, first, __ffs(same) - 1) + before;
-    }
-    __syncthreads();
-    {
-        const u32 d = threadIdx.x;
-        u32 all;
-        u32 run = block_exclusive(totals[d], tmp, &all) + counts[d * tiles + blockIdx.x];
-        for (u32 i = 0; i < kSortBlock / 32; ++i)
-        {
-            const u32 c = at[i][d];
-            at[i][d] = run;
-            run += c;
-        }
+        const bool is = in.key(i, size, key[k]);
+        place[k] = is ? in.place(i) : 0;
+        held |= static_cast<u32>(is) << k;
     }
     __syncthreads();
 #pragma unroll
     for (u32 k = 0; k < kSortRounds; ++k)
+        rank[k] = warp_rank(in.digit(key[k]), held >> k & 1, in.bits, at[w]);
+    const u32 d = threadIdx.x;
+    u32 all;
+    u32 run = digits_exclusive(totals[d], tmp, &all) + counts[d * in.tiles + blockIdx.x];
+    for (u32 i = 0; i < kSortBlock / 32; ++i)
     {
-        const u32 i = base + k * 32 + lane;
-        if (i < n)
+        const u32 c = at[i][d];
+        at[i][d] = run;
+        run += c;
+    }
+    if (held_count && blockIdx.x == 0 && threadIdx.x == 0)
+        *held_count = all;
+    __syncthreads();
+#pragma unroll
+    for (u32 k = 0; k < kSortRounds; ++k)
+        if (held >> k & 1)
         {
-            const u32 to = at[w][key[k] >> shift & (kBins - 1)] + rank[k];
+            const u32 to = at[w][in.digit(key[k])] + rank[k];
             keys[to] = key[k];
-            places[to] = in.place(i);
+            places[to] = place[k];
         }
-    }
 }
+
+// ---------------------------------------------------------------------------------------------- sums of the segments
 
 struct Segments
 {
     const u32* keys;
     const u32* places;
-    u32 n, vocabulary, chunk, chunks;
-    u32 columns;  // vectors of a row
-    u32 slices;   // of `lanes` vectors each
+    const u32* count;  // of the sorted list
+    u32 chunk, chunks;  // a multiple of eight entries; as many as the list could fill
+    u32 columns;        // vectors of a row
     float scale;
     u64 width, grad_stride;
     float* partial;  // [chunks, 2, width]: of the token that comes into the chunk, of the one that goes on after it
@@ -185,26 +386,25 @@ __device__ __forceinline__ void store_scaled(T* to, const float* sum, float scal
     *reinterpret_cast<Vec<T, VE>*>(to) = o;
 }
 
-/// `lanes` threads (a power of two up to 32) take a chunk's slice of columns, one vector each.
+/// A thread for each chunk and vector of columns; eight gradient rows are under way at a time.
 template<class T, int VE>
-__global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* __restrict__ grad, T* __restrict__ out,
-                                                     u32 lanes)
+__global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* __restrict__ grad, T* __restrict__ out)
 {
-    const u64 item = (static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
-    if (item >= static_cast<u64>(a.chunks) * a.slices)
+    constexpr u32 U = 8;
+    const u64 id = static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const u64 items = static_cast<u64>(a.chunks) * a.columns;
+    if (id >= items)
         return;
-    const u32 c = static_cast<u32>(item / a.slices);
-    const u32 column = static_cast<u32>(item % a.slices) * lanes + (threadIdx.x & (lanes - 1));
-    if (column >= a.columns)
+    const u32 c = items >> 32 ? static_cast<u32>(id / a.columns) : static_cast<u32>(id) / a.columns;
+    const u64 offset = (id - static_cast<u64>(c) * a.columns) * VE;
+    const u32 n = *a.count, begin = c * a.chunk;
+    if (begin >= n)
         return;
-    const u64 offset = static_cast<u64>(column) * VE;
-    const u32 begin = c * a.chunk, end = min(begin + a.chunk, a.n);
+    const u32 end = min(begin + a.chunk, n);
     u32 current = a.keys[begin];
     bool comes_in = begin && a.keys[begin - 1] == current;
     float sum[VE] = {};
     auto flush = [&](bool goes_on) {
-        if (current >= a.vocabulary)
-            return;
         if (!comes_in && !goes_on)
             store_scaled<T, VE>(out + current * a.width + offset, sum, a.scale);
         else
@@ -215,67 +415,130 @@ __global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* 
                 to[k] = sum[k];
         }
     };
-    for (u32 i = begin; i < end; ++i)
+    for (u32 i = begin; i < end; i += U)
     {
-        const u32 key = a.keys[i];
-        if (key != current)
-        {
-            flush(false);
-            comes_in = false;
-            current = key;
+        u32 key[U], place[U];  // the arrays are padded to whole groups
 #pragma unroll
-            for (int k = 0; k < VE; ++k)
-                sum[k] = 0;
+        for (u32 k = 0; k < U; k += 4)
+        {
+            *reinterpret_cast<uint4*>(key + k) = *reinterpret_cast<const uint4*>(a.keys + i + k);
+            *reinterpret_cast<uint4*>(place + k) = *reinterpret_cast<const uint4*>(a.places + i + k);
         }
-        if (key < a.vocabulary)
-        {
-            const Vec<T, VE> g = *reinterpret_cast<const Vec<T, VE>*>(grad + a.places[i] * a.grad_stride + offset);
+        Vec<T, VE> g[U];
 #pragma unroll
-            for (int k = 0; k < VE; ++k)
-                sum[k] += to_f32(g.v[k]);
+        for (u32 k = 0; k < U; ++k)
+            if (i + k < end)
+                g[k] = *reinterpret_cast<const Vec<T, VE>*>(grad + place[k] * a.grad_stride + offset);
+#pragma unroll
+        for (u32 k = 0; k < U; ++k)
+        {
+            if (i + k >= end)
+                break;
+            if (key[k] != current)
+            {
+                flush(false);
+                comes_in = false;
+                current = key[k];
+#pragma unroll
+                for (int j = 0; j < VE; ++j)
+                    sum[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                sum[j] += to_f32(g[k].v[j]);
         }
     }
-    flush(end < a.n && a.keys[end] == current);
+    flush(end < n && a.keys[end] == current);
 }
 
-/// A block for each chunk out of which a token goes on that did not come into it: adds its partial sums in chunk order.
+constexpr u32 kJoinColumns = 128;
+
+/// A block for each chunk out of which a token goes on that did not come into it, and 128 columns: its warps take the
+/// partial sums of every eighth chunk, and their sums are added in the warps' order.
 template<class T>
 __global__ void __launch_bounds__(256) k_segment_join(const Segments a, T* __restrict__ out)
 {
-    const u32 c = blockIdx.x;
-    const u32 begin = c * a.chunk, end = begin + a.chunk;
-    if (end >= a.n)
+    __shared__ float sums[8][kJoinColumns];
+    const u32 c = blockIdx.x, n = *a.count;
+    const u64 begin = static_cast<u64>(c) * a.chunk, end = begin + a.chunk;
+    if (end >= n)
         return;
     const u32 key = a.keys[end];
-    if (key >= a.vocabulary || a.keys[end - 1] != key || (begin && a.keys[begin - 1] == key))
+    if (a.keys[end - 1] != key || (begin && a.keys[begin - 1] == key))
         return;
-    for (u64 col = threadIdx.x; col < a.width; col += blockDim.x)
+    u32 more = 1;  // chunks that the token comes into
+    for (;;)
     {
-        float sum = a.partial[(static_cast<u64>(c) * 2 + 1) * a.width + col];
-        for (u32 i = c + 1; i < a.chunks && a.keys[static_cast<u64>(i) * a.chunk] == key; ++i)
-            sum += a.partial[static_cast<u64>(i) * 2 * a.width + col];
-        out[key * a.width + col] = from_f32<T>(sum * a.scale);
+        const u64 first = (static_cast<u64>(c) + 1 + more + threadIdx.x) * a.chunk;
+        const u32 got = __syncthreads_count(first < n && a.keys[first] == key);
+        more += got;
+        if (got < blockDim.x)
+            break;
+    }
+    const u32 lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const u64 column = static_cast<u64>(blockIdx.y) * kJoinColumns + lane;
+    float sum[kJoinColumns / 32] = {};
+#pragma unroll 4
+    for (u32 i = w; i <= more; i += 8)
+    {
+        // the first partial sum is of the token that goes on, the others of the one that comes in
+        const float* from = a.partial + ((static_cast<u64>(c) + i) * 2 + (i == 0)) * a.width + column;
+#pragma unroll
+        for (u32 k = 0; k < kJoinColumns / 32; ++k)
+            if (column + k * 32 < a.width)
+                sum[k] += from[k * 32];
+    }
+#pragma unroll
+    for (u32 k = 0; k < kJoinColumns / 32; ++k)
+        sums[w][k * 32 + lane] = sum[k];
+    __syncthreads();
+    const u64 col = static_cast<u64>(blockIdx.y) * kJoinColumns + threadIdx.x;
+    if (threadIdx.x < kJoinColumns && col < a.width)
+    {
+        float all = 0;
+        for (u32 i = 0; i < 8; ++i)
+            all += sums[i][threadIdx.x];
+        out[key * a.width + col] = from_f32<T>(all * a.scale);
     }
 }
 
+// ---------------------------------------------------------------------------------------------- lookup
+
+constexpr u32 kLookupRows = 4;
+
+/// A thread for each vector of columns and four rows.
 template<class T, int VE>
 __global__ void __launch_bounds__(256) k_lookup(const b2_embedding_args a, const T* __restrict__ weight, u64 stride,
                                                 T* __restrict__ rows, u32 columns)
 {
-    const u64 items = a.count * columns;
-    for (u64 i = static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x; i < items;
-         i += static_cast<u64>(gridDim.x) * blockDim.x)
-    {
-        const u64 r = i / columns, offset = (i % columns) * VE;
-        const long long t = token_at(a.tokens, a.token_bits, r);
-        Vec<T, VE> x;
-        const bool in = t >= 0 && t < static_cast<long long>(a.vocabulary);
-        if (in)
-            x = *reinterpret_cast<const Vec<T, VE>*>(weight + t * stride + offset);
+    const u64 id = static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const u64 groups = (a.count + kLookupRows - 1) / kLookupRows, items = groups * columns;
+    if (id >= items)
+        return;
+    const u64 group = items >> 32 ? id / columns : static_cast<u32>(id) / columns;
+    const u64 offset = (id - group * columns) * VE;
+    long long t[kLookupRows];
+    Vec<T, VE> x[kLookupRows];
 #pragma unroll
-        for (int k = 0; k < VE; ++k)
-            x.v[k] = from_f32<T>(in ? to_f32(x.v[k]) * a.scale : t < 0 ? 0.f : nanf(""));
-        *reinterpret_cast<Vec<T, VE>*>(rows + r * a.width + offset) = x;
+    for (u32 k = 0; k < kLookupRows; ++k)
+    {
+        const u64 r = group * kLookupRows + k;
+        t[k] = r < a.count ? token_at(a.tokens, a.token_bits, r) : -1;
+    }
+#pragma unroll
+    for (u32 k = 0; k < kLookupRows; ++k)
+        if (t[k] >= 0 && t[k] < static_cast<long long>(a.vocabulary))
+            x[k] = *reinterpret_cast<const Vec<T, VE>*>(weight + t[k] * stride + offset);
+#pragma unroll
+    for (u32 k = 0; k < kLookupRows; ++k)
+    {
+        const u64 r = group * kLookupRows + k;
+        const bool in = t[k] >= 0 && t[k] < static_cast<long long>(a.vocabulary);
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+            x[k].v[j] = from_f32<T>(in ? to_f32(x[k].v[j]) * a.scale : t[k] < 0 ? 0.f : nanf(""));
+        if (r < a.count)
+            *reinterpret_cast<Vec<T, VE>*>(rows + r * a.width + offset) = x[k];
     }
 }
 
@@ -305,23 +568,30 @@ void dispatch_vector(int ve, F&& f)
     }
 }
 
-/// The workspace of a backward call.
+/// The layout of a backward call and its workspace.
 struct Plan
 {
-    u32 n, tiles, passes, chunk, chunks;
-    size_t keys[2], places[2], counts, totals, partial, bytes;
+    u32 n, passes, bits, tiles, chunk, chunks;
+    bool cluster;
+    size_t keys[2], places[2], counts, totals, held, partial, bytes;
 };
 
 Plan plan_of(const b2_embedding_args& a)
 {
     Plan p{};
     p.n = static_cast<u32>(a.count);
-    p.tiles = (p.n + kSortTile - 1) / kSortTile;
     u32 bits = 1;
-    while (a.vocabulary >> bits)
+    while (bits < 31 && (a.vocabulary - 1) >> bits)
         ++bits;
-    p.passes = (bits + kDigitBits - 1) / kDigitBits;
-    p.chunk = 32;
+    p.passes = (bits + 7) / 8;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    p.cluster = p.n <= kClusterMost;
+    p.tiles = (p.n + kSortTile - 1) / kSortTile;
+    // chunks as short as leaves a thread for each of 1,024 in an SM: long enough to keep partial sums few, short enough
+    // to fill the device (columns counted as vectors of 16 bytes)
+    const u64 columns = std::max<u64>(1, a.width * size_of(a.dtype) / 16);
+    const u64 even = a.count * columns / (148 * 1024);
+    p.chunk = static_cast<u32>(std::min<u64>(256, std::max<u64>(8, (even + 7) / 8 * 8)));
     p.chunks = (p.n + p.chunk - 1) / p.chunk;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -329,16 +599,79 @@ Plan plan_of(const b2_embedding_args& a)
         at = (at + bytes + 255) & ~size_t{255};
         return was;
     };
-    for (int k = 0; k < 2; ++k)
+    const size_t list = (static_cast<size_t>(p.n) + 8) * 4;  // the sums read it in whole groups of eight
+    for (int k = 0; k < (p.cluster || p.passes == 1 ? 1 : 2); ++k)
     {
-        p.keys[k] = take(static_cast<size_t>(p.n) * 4);
-        p.places[k] = take(static_cast<size_t>(p.n) * 4);
+        p.keys[k] = take(list);
+        p.places[k] = take(list);
     }
-    p.counts = take(static_cast<size_t>(p.tiles) * kBins * 4);
-    p.totals = take(kBins * 4);
+    if (!p.cluster)
+    {
+        p.counts = take(static_cast<size_t>(p.tiles) * kBins * 4);
+        p.totals = take(kBins * 4);
+    }
+    p.held = take(4);
     p.partial = take(static_cast<size_t>(p.chunks) * 2 * a.width * 4);
     p.bytes = at;
     return p;
+}
+
+/// Sorts the tokens' places and sets the table's gradient to zero; the sorted list and its length are s.keys, s.places
+/// and s.count.
+void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, char* ws, const Zeros& zeros, Segments& s,
+                 cudaStream_t st)
+{
+    auto words = [&](size_t at) { return reinterpret_cast<u32*>(ws + at); };
+    const Tokens tokens{a.tokens, a.token_bits, static_cast<u32>(a.vocabulary)};
+    const u64 vectors = zeros.bytes / 16 + 1;
+    s.count = words(p.held);
+    if (p.cluster)
+    {
+        const u32 share = std::max(1u, (p.n + kClusterBlocks * kClusterThreads - 1) / (kClusterBlocks * kClusterThreads)) *
+                          kClusterThreads;
+        const size_t shared = cluster_bytes(share);
+        static std::once_flag once[64];
+        std::call_once(once[ctx.device & 63], [&] {
+            B2_CUDA(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(cluster_bytes(kClusterThreads * kClusterRounds))));
+        });
+        // a block of zeros for each SM that the sort leaves, while there is a vector for each thread
+        const u64 most = static_cast<u64>(ctx.sms) / kClusterBlocks * kClusterBlocks - kClusterBlocks;
+        const u64 want = (vectors + kClusterThreads - 1) / kClusterThreads;
+        const u64 blocks = (std::min(most, want) + kClusterBlocks - 1) / kClusterBlocks * kClusterBlocks;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(kClusterBlocks + blocks));
+        cfg.blockDim = dim3(kClusterThreads);
+        cfg.dynamicSmemBytes = shared;
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kClusterBlocks;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        s.keys = words(p.keys[0]);
+        s.places = words(p.places[0]);
+        B2_CUDA(cudaLaunchKernelEx(&cfg, k_sort_cluster, tokens, p.n, share, p.passes, p.bits, words(p.keys[0]),
+                                   words(p.places[0]), words(p.held), zeros));
+        return;
+    }
+    Pass in{tokens, nullptr, nullptr, nullptr, p.n, 0, p.bits, p.tiles};
+    for (u32 i = 0; i < p.passes; ++i)
+    {
+        in.shift = i * p.bits;
+        u32* const keys = words(p.keys[i & 1]);
+        u32* const places = words(p.places[i & 1]);
+        const unsigned extra = i == 0 ? grid_for(vectors, kSortBlock, static_cast<unsigned>(ctx.sms) * 8) : 0;
+        k_sort_count<<<p.tiles + extra, kSortBlock, 0, st>>>(in, words(p.counts), zeros);
+        k_sort_scan<<<kBins, kSortBlock, 0, st>>>(words(p.counts), p.tiles, words(p.totals));
+        k_sort_scatter<<<p.tiles, kSortBlock, 0, st>>>(in, words(p.counts), words(p.totals), keys, places,
+                                                       i == 0 ? words(p.held) : nullptr);
+        in.keys = s.keys = keys;
+        in.places = s.places = places;
+        in.count = s.count;
+    }
+    B2_CUDA(cudaGetLastError());
 }
 
 void check_args(b2_ctx* ctx, const b2_embedding_args* a, const char* what)
@@ -375,8 +708,10 @@ b2_status b2_embedding(b2_ctx* ctx, const b2_embedding_args* args, const void* w
             const int ve = vector_width<T>(a.width, weight_stride, weight, rows);
             dispatch_vector<T>(ve, [&]<int VE>() {
                 const u32 columns = static_cast<u32>(a.width / VE);
-                const unsigned grid = grid_for(a.count * columns, 256, static_cast<unsigned>(ctx->sms) * 16);
-                k_lookup<T, VE><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                const u64 blocks = ((a.count + kLookupRows - 1) / kLookupRows * columns + 255) / 256;
+                if (blocks >= 1ull << 31)
+                    throw Error(B2_CAPACITY, "b2_embedding: too many rows for one call");
+                k_lookup<T, VE><<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
                     a, static_cast<const T*>(weight), weight_stride, static_cast<T*>(rows), columns);
             });
             B2_CUDA(cudaGetLastError());
@@ -402,31 +737,15 @@ b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, cons
                 throw Error(B2_CAPACITY, "b2_embedding_backward: the workspace is too small or not 16-byte aligned");
             const OnDevice on(ctx->device);
             const cudaStream_t st = static_cast<cudaStream_t>(stream);
-            B2_CUDA(cudaMemsetAsync(grad_weight, 0, a.vocabulary * a.width * sizeof(T), st));
+            const Zeros zeros{grad_weight, a.vocabulary * a.width * sizeof(T)};
             if (!a.count)
-                return;
-            char* ws = static_cast<char*>(workspace);
-            u32* keys[2] = {reinterpret_cast<u32*>(ws + p.keys[0]), reinterpret_cast<u32*>(ws + p.keys[1])};
-            u32* places[2] = {reinterpret_cast<u32*>(ws + p.places[0]), reinterpret_cast<u32*>(ws + p.places[1])};
-            u32* counts = reinterpret_cast<u32*>(ws + p.counts);
-            u32* totals = reinterpret_cast<u32*>(ws + p.totals);
-            Keys in{a.tokens, nullptr, nullptr, a.token_bits, static_cast<u32>(a.vocabulary)};
-            for (u32 i = 0; i < p.passes; ++i)
             {
-                const u32 shift = i * kDigitBits;
-                k_sort_count<<<p.tiles, kSortBlock, 0, st>>>(in, p.n, shift, p.tiles, counts);
-                k_sort_scan<<<kBins, kSortBlock, 0, st>>>(counts, p.tiles, totals);
-                k_sort_scatter<<<p.tiles, kSortBlock, 0, st>>>(in, p.n, shift, p.tiles, counts, totals, keys[i & 1],
-                                                               places[i & 1]);
-                in.tokens = nullptr;
-                in.keys = keys[i & 1];
-                in.places = places[i & 1];
+                B2_CUDA(cudaMemsetAsync(zeros.p, 0, zeros.bytes, st));
+                return;
             }
+            char* ws = static_cast<char*>(workspace);
             Segments s{};
-            s.keys = in.keys;
-            s.places = in.places;
-            s.n = p.n;
-            s.vocabulary = static_cast<u32>(a.vocabulary);
+            sort_tokens(*ctx, a, p, ws, zeros, s, st);
             s.chunk = p.chunk;
             s.chunks = p.chunks;
             s.scale = a.scale;
@@ -436,18 +755,19 @@ b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, cons
             const int ve = vector_width<T>(a.width, grad_stride, grad, grad_weight);
             dispatch_vector<T>(ve, [&]<int VE>() {
                 s.columns = static_cast<u32>(a.width / VE);
-                u32 lanes = 1;
-                while (lanes < 32 && lanes < s.columns)
-                    lanes *= 2;
-                s.slices = (s.columns + lanes - 1) / lanes;
-                const u64 threads = static_cast<u64>(s.chunks) * s.slices * lanes;
-                const u64 blocks = (threads + 255) / 256;
+                const u64 blocks = (static_cast<u64>(s.chunks) * s.columns + 255) / 256;
                 if (blocks >= 1ull << 31)
                     throw Error(B2_CAPACITY, "b2_embedding_backward: too many gradients for one call");
-                k_segment_sum<T, VE><<<static_cast<unsigned>(blocks), 256, 0, st>>>(
-                    s, static_cast<const T*>(grad), static_cast<T*>(grad_weight), lanes);
+                k_segment_sum<T, VE><<<static_cast<unsigned>(blocks), 256, 0, st>>>(s, static_cast<const T*>(grad),
+                                                                                  static_cast<T*>(grad_weight));
             });
-            k_segment_join<T><<<s.chunks, 256, 0, st>>>(s, static_cast<T*>(grad_weight));
+            if (s.chunks > 1)
+            {
+                const dim3 grid(s.chunks, static_cast<unsigned>((a.width + kJoinColumns - 1) / kJoinColumns));
+                if (grid.y > 65535)
+                    throw Error(B2_CAPACITY, "b2_embedding_backward: rows of more than 8,388,480 columns");
+                k_segment_join<T><<<grid, 256, 0, st>>>(s, static_cast<T*>(grad_weight));
+            }
             B2_CUDA(cudaGetLastError());
         });
     });
