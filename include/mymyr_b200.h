@@ -443,7 +443,7 @@ typedef struct b2_logprobs_args {
     float* logprob;          /* [rows]; required with tokens */
     float* entropy;          /* [rows] */
     float* stats;            /* [rows, 4], 16-byte aligned, or NULL: what the backward pass needs of a row (its largest
-                                logit, the log of its sum of exp((x - largest) / T), its entropy, unused) */
+                                logit, the log of its sum of exp((x - largest) / T), its entropy, that sum's log2) */
     float* top_logprobs;     /* [rows, top], from the best down; -inf past the row's tokens */
     int64_t* top_tokens;     /* [rows, top]; equal logits in index order; -1 past the row's tokens */
 } b2_logprobs_args;
@@ -456,7 +456,8 @@ b2_status b2_logprobs(b2_ctx* ctx, const b2_logprobs_args* args, void* stream);
 
 /* The gradient of the logits from those of logprob and entropy (either may be NULL), given the call's arguments with
  * the stats that it wrote. grad_logits: same type as the logits, dense rows grad_stride apart, or ragged
- * [width] (elements outside every row are not written). Zero for masked tokens and rows that leave nothing. */
+ * [width] (written whole: zeros before the first row and after the last). Zero for masked tokens and rows that leave
+ * nothing. Offsets must not decrease here: rows that overlap would overwrite one another. */
 b2_status b2_logprobs_backward(b2_ctx* ctx, const b2_logprobs_args* args, const float* grad_logprob,
                                const float* grad_entropy, void* grad_logits, uint64_t grad_stride, void* stream);
 

@@ -55,32 +55,6 @@ __host__ __device__ __forceinline__ u32 mix(u32 x)
     return x;
 }
 
-/// Two 32-bit numbers in a register pair, for the packed arithmetic of sm_100 (each half rounds as the plain operation).
-struct Two
-{
-    u64 v;
-    Two() = default;
-    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ float2 get() const
-    {
-        float2 f;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-        return f;
-    }
-};
-__device__ __forceinline__ Two operator*(Two a, Two b)
-{
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two operator+(Two a, Two b)
-{
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-
 /// Eight consecutive elements: one 32-byte or 16-byte access.
 __device__ __forceinline__ void load8(const float* p, float (&x)[8])
 {

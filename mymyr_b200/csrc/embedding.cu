@@ -122,8 +122,8 @@ __device__ __forceinline__ u32 digits_exclusive(u32 v, u32* tmp, u32* total)
 // ---------------------------------------------------------------------------------------------- sort in one cluster
 
 constexpr u32 kClusterBlocks = 8, kClusterThreads = 1024, kClusterWarps = 32;
-constexpr u32 kClusterRounds = 8;                                                      // keys of a thread
-constexpr u32 kClusterMost = kClusterBlocks * kClusterThreads * kClusterRounds;        // 65,536 keys
+constexpr u32 kClusterRounds = 4;                                                      // keys of a thread
+constexpr u32 kClusterMost = kClusterBlocks * kClusterThreads * kClusterRounds;        // 32,768 keys
 
 /// The shared memory of a block: two sets of keys and places, the warps' counts of each digit, and their sums.
 constexpr size_t cluster_bytes(u32 share)

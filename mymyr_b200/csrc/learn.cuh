@@ -35,6 +35,39 @@ __device__ __forceinline__ f16 from_f32<f16>(float x)
     return __float2half_rn(x);
 }
 
+/// Two 32-bit numbers in a register pair, for the packed arithmetic of sm_100 (each half rounds as the plain operation).
+struct Two
+{
+    u64 v;
+    Two() = default;
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float2 get() const
+    {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b)
+{
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b)
+{
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+__device__ __forceinline__ Two fma(Two a, Two b, Two c)
+{
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 inline size_t size_of(int32_t dtype) { return dtype == B2_F32 ? 4 : 2; }
 
 /// Calls f.template operator()<T>() for the element type.

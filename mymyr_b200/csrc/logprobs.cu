@@ -145,14 +145,14 @@ struct Sums
 /// The results of a row from its joined sums (s about ref): the same arithmetic on every path.
 struct Row
 {
-    float ref, log_s, entropy, inv_t;
+    float ref, log2_s, log_s, entropy, inv_t;
     bool dead, bad;
     __device__ __forceinline__ Row(const Sums& a, float inv_temperature)
         : ref(a.ref), inv_t(inv_temperature), dead(a.best == -kInf && a.s == a.s), bad(a.s != a.s)
     {
-        const float l2 = __log2f(a.s);
-        log_s = dead ? -kInf : l2 * kLn2;
-        entropy = dead ? 0.f : (l2 - a.t / a.s) * kLn2;
+        log2_s = __log2f(a.s);
+        log_s = dead ? -kInf : log2_s * kLn2;
+        entropy = dead ? 0.f : (log2_s - a.t / a.s) * kLn2;
     }
     __device__ __forceinline__ float logp(float x) const
     {
@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_row(const Forward& a, u64 r, const Row& ro
         a.logprob[r] = token < 0 ? 0.f : token >= len ? nanf("") : row.logp(logit);
     a.entropy[r] = row.entropy;
     if (a.stats)
-        reinterpret_cast<float4*>(a.stats)[r] = make_float4(row.dead ? -kInf : row.ref, row.log_s, row.entropy, 0.f);
+        reinterpret_cast<float4*>(a.stats)[r] = make_float4(row.dead ? -kInf : row.ref, row.log_s, row.entropy, row.log2_s);
 }
 
 __device__ __forceinline__ void store_top(const Forward& a, u64 r, u32 i, const Row& row, u64 key)
@@ -326,36 +326,62 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const Forward a)
     }
 }
 
-/// One element of the gradient of the logits.
+/// The gradient of a row's logits: with y = log2 of the probability p, -p (gl + ge (ln p + entropy)) / temperature is
+/// p (a + b y), and the given token's own logit gets gl / temperature more.
 struct Slope
 {
-    float ref, log_s, entropy, inv_t, gl, ge;
+    float ref, c, shift, a, b, own;
     bool dead;
-    __device__ __forceinline__ Slope(const Backward& a, u64 r, long long& token, u32 len) : inv_t(a.inv_t)
+    __device__ __forceinline__ Slope(const Backward& g, u64 r, long long& token, u32 len)
     {
-        const float4 st = reinterpret_cast<const float4*>(a.stats)[r];
-        ref = st.x, log_s = st.y, entropy = st.z;
+        const float4 st = reinterpret_cast<const float4*>(g.stats)[r];
+        ref = st.x;
         dead = st.x == -kInf;
-        gl = a.grad_logprob ? a.grad_logprob[r] : 0.f;
-        ge = a.grad_entropy ? a.grad_entropy[r] : 0.f;
-        token = a.grad_logprob ? token_at(a.tokens, a.token_bits, r) : -1;
-        if (a.grad_logprob)
+        c = g.inv_t * kLog2e;
+        shift = -st.w;
+        float gl = g.grad_logprob ? g.grad_logprob[r] : 0.f;
+        const float ge = g.grad_entropy ? g.grad_entropy[r] : 0.f;
+        token = g.grad_logprob ? token_at(g.tokens, g.token_bits, r) : -1;
+        if (g.grad_logprob)
             gl = token < 0 ? 0.f : token >= len ? nanf("") : gl;
+        own = gl * g.inv_t;
+        a = st.y == st.y ? -fmaf(ge, st.z, gl) * g.inv_t : st.y;  // NaN for all where the row held one
+        b = -ge * kLn2 * g.inv_t;
     }
-    __device__ __forceinline__ float operator()(float x, bool is_token) const
+    /// Without the token's own part. Where y is below -200, p is 0: minus infinity must not come in.
+    __device__ __forceinline__ float2 of(float x0, float x1) const
     {
-        // below -200 the probability is 0: minus infinity must not come in
-        const float lp = fmaxf((x - ref) * inv_t - log_s, -200.f), p = exp2_approx(lp * kLog2e);
-        const float g = fmaf(-p, fmaf(ge, lp + entropy, gl), is_token ? gl : 0.f) * inv_t;
-        return log_s == log_s ? g : log_s;
+        const float2 y = fma(Two(x0, x1) + Two(-ref, -ref), Two(c, c), Two(shift, shift)).get();
+        const float y0 = fmaxf(y.x, -200.f), y1 = fmaxf(y.y, -200.f);
+        const Two p(exp2_approx(y0), exp2_approx(y1));
+        return (p * fma(Two(y0, y1), Two(b, b), Two(a, a))).get();
     }
 };
+
+/// Zeros for the places of a ragged vector before its first row and after its last.
+template<class T>
+__device__ __forceinline__ void zero_outside(const Backward& a)
+{
+    if (!a.rows.offsets)
+        return;
+    const long long n = static_cast<long long>(a.rows.width);
+    const long long head = min(max(token_at(a.rows.offsets, a.rows.offsets_bits, 0), 0ll), n);
+    const long long tail = min(max(token_at(a.rows.offsets, a.rows.offsets_bits, a.count), 0ll), n);
+    T* const dx = static_cast<T*>(a.grad);
+    const long long thread = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const long long threads = static_cast<long long>(gridDim.x) * blockDim.x;
+    for (long long j = thread; j < head; j += threads)
+        dx[j] = from_f32<T>(0.f);
+    for (long long j = tail + thread; j < n; j += threads)
+        dx[j] = from_f32<T>(0.f);
+}
 
 template<class T, int G>
 __global__ void __launch_bounds__(128) k_logprobs_backward_short(const Backward a)
 {
     const u32 lane = threadIdx.x & (G - 1);
     const u64 r = (static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x) / G;
+    zero_outside<T>(a);
     if (r >= a.count)
         return;
     u64 begin, mask_begin;
@@ -368,7 +394,10 @@ __global__ void __launch_bounds__(128) k_logprobs_backward_short(const Backward 
     const Slope slope(a, r, token, len);
 #pragma unroll 4
     for (u32 j = lane; j < len; j += G)
-        dx[j] = from_f32<T>(slope.dead || (mask && !mask[j]) ? 0.f : slope(to_f32(x[j]), j == token));
+    {
+        const bool none = slope.dead || (mask && !mask[j]);
+        dx[j] = from_f32<T>(none ? 0.f : slope.of(to_f32(x[j]), 0.f).x + (j == token ? slope.own : 0.f));
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- long rows
@@ -449,22 +478,47 @@ __device__ __forceinline__ float max_of(const float (&x)[N])
     return m;
 }
 
-/// What a thread knows of the logits that it read: their sums, and the vector of the first of their largest.
+/// What a thread knows of the logits that it read: their sums (in two halves), and the vector of the first of their
+/// largest.
 template<int VE>
 struct Scan
 {
-    Sums sum;
+    float ref = kLowest, best = -kInf;
+    Two s{0.f, 0.f}, t{0.f, 0.f};
     u32 at = 0;
+    __device__ __forceinline__ Sums sums(float c) const
+    {
+        const float2 a = s.get(), b = t.get();
+        Sums r;
+        r.ref = ref, r.s = a.x + a.y, r.t = b.x + b.y, r.best = best;
+        return r;
+    }
     __device__ __forceinline__ void add(const float (&x)[VE], u32 i, float c, float ahead)
     {
         const float m = max_of(x);
-        at = m > sum.best ? i : at;
-        sum.best = fmaxf(sum.best, m);
-        if (m > sum.ref + ahead)
-            sum.move(m, c);
+        at = m > best ? i : at;
+        best = fmaxf(best, m);
+        if (m > ref + ahead)
+        {
+            const float2 a = s.get(), b = t.get();
+            Sums one, two;
+            one.ref = two.ref = ref;
+            one.s = a.x, two.s = a.y, one.t = b.x, two.t = b.y;
+            one.move(m, c);
+            two.move(m, c);
+            ref = m;
+            s = Two(one.s, two.s);
+            t = Two(one.t, two.t);
+        }
+        const Two c2(c, c), back(-ref, -ref);
 #pragma unroll
-        for (int k = 0; k < VE; ++k)
-            sum.add(x[k], c);
+        for (int k = 0; k < VE; k += 2)
+        {
+            const float2 d = ((Two(x[k], x[k + 1]) + back) * c2).get();
+            const Two e(exp2_approx(d.x), exp2_approx(d.y));
+            s = s + e;
+            t = fma(e, Two(fmaxf(d.x, -200.f), fmaxf(d.y, -200.f)), t);  // e is 0 there: no minus infinity in t
+        }
     }
 };
 
@@ -492,8 +546,11 @@ template<class T, bool MASK, int NW>
 __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 cluster)
 {
     constexpr int VE = kVec<T>, N = NW * 32, U = 4;
+    constexpr u32 kFound = N;
     __shared__ u64 lists[NW * kListKeys];
     __shared__ u64 threshold_keys[kListKeys];
+    __shared__ u64 candidates[kFound];
+    __shared__ u32 held_keys, found;
     __shared__ float4 sums[NW];  // of each warp
     __shared__ float4 block_sums;
     __shared__ u64 block_list[kListKeys];
@@ -556,7 +613,7 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
         scan.add(v, i, c, ahead);
     }
     // the block's sums about its largest logit
-    Sums sum = scan.sum;
+    Sums sum = scan.sums(c);
     float best = sum.best;
 #pragma unroll
     for (int o = 16; o; o /= 2)
@@ -576,46 +633,86 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
     if (a.top)
     {
         // the threads' best; the top-th of them bounds what can be among the row's best
-        list = block_merge<NW>(warp_sort(key_of(scan.sum.best, scan.at)), lists);
+        list = block_merge<NW>(warp_sort(key_of(scan.best, scan.at)), lists);
         if (w == 0)
+        {
             threshold_keys[lane] = lane < a.top ? list : 0;
+            const u32 held = __popc(__ballot_sync(~0u, lane < a.top && list));
+            if (lane == 0)
+            {
+                held_keys = held;
+                found = 0;
+            }
+        }
     }
     __syncthreads();
     if (a.top)
     {
-        list = 0;
+        // the logits of the best threads (every N-th vector), those that reach the bound; as many as a thread can hold
+        // each are seldom more than the alternatives themselves
         const u64 bound = threshold_keys[a.top - 1];
-        for (u32 k = w; k < a.top && threshold_keys[k]; k += NW)
+        const u32 each = (last - first + N - 1) / N, pairs = min(a.top, held_keys) * each;
+        for (u32 p = tid; p < pairs; p += N)
         {
-            // the logits of the k-th best thread: every N-th vector
-            const u32 owner = (index_of(threshold_keys[k]) - first) % N;
-            for (u32 j0 = first + owner; j0 < last; j0 += 32 * N)
+            const u32 j = first + (index_of(threshold_keys[p / each]) - first) % N + p % each * N;
+            if (j >= last)
+                continue;
+            float v[VE];
+            row.load_any(j, v);
+            if (key_of(max_of(v), j) < bound)
+                continue;
+            for (int q = 0; q < VE; ++q)
             {
-                const u32 j = j0 + lane * N;
-                float v[VE];
-                bool any = false;
-                if (j < last && j >= j0)
+                const u64 key = key_of(v[q], j * VE - row.shift + q);
+                if (!key || (key | ~0u) < bound)  // a smaller logit than the bound's
+                    continue;
+                const u32 to = atomicAdd(&found, 1u);
+                if (to < kFound)
+                    candidates[to] = key;
+            }
+        }
+        __syncthreads();
+        if (found <= kFound)
+        {
+            // sorted by as many warps as they fill
+            const u32 at = w * 32 + lane;
+            list = w * 32 < found || w == 0 ? warp_sort(at < found ? candidates[at] : 0) : 0;
+            if (found > 32)
+                list = block_merge<NW>(list, lists);
+        }
+        else
+        {
+            // a row of many equal ones: each warp takes best threads in turn and keeps a sorted list
+            list = 0;
+            for (u32 k = w; k < held_keys && k < a.top; k += NW)
+            {
+                const u32 owner = (index_of(threshold_keys[k]) - first) % N;
+                for (u32 j0 = first + owner; j0 < last; j0 += 32 * N)
                 {
-                    row.load_any(j, v);
-                    any = key_of(max_of(v), j) >= bound;
-                }
-                for (u32 more = __ballot_sync(~0u, any); more; more &= more - 1)
-                {
-                    const int src = __ffs(more) - 1;
-                    const u32 at = __shfl_sync(~0u, j, src) * VE - row.shift;
-#pragma unroll
-                    for (int q = 0; q < VE; ++q)
+                    const u32 j = j0 + lane * N;
+                    float v[VE];
+                    bool any = false;
+                    if (j < last)
                     {
-                        const float y = __shfl_sync(~0u, v[q], src);
-                        const u64 key = key_of(y, at + q);
-                        // warp-uniform: the list's last place is the bound for the rest
-                        if (key > __shfl_sync(~0u, list, 31))
-                            list = warp_insert(list, key);
+                        row.load_any(j, v);
+                        any = key_of(max_of(v), j) >= bound;
+                    }
+                    for (u32 more = __ballot_sync(~0u, any); more; more &= more - 1)
+                    {
+                        const int src = __ffs(more) - 1;
+                        const u32 at = __shfl_sync(~0u, j, src) * VE - row.shift;
+#pragma unroll
+                        for (int q = 0; q < VE; ++q)
+                        {
+                            const u64 key = key_of(__shfl_sync(~0u, v[q], src), at + q);
+                            if (key > __shfl_sync(~0u, list, 31))  // the same for the whole warp
+                                list = warp_insert(list, key);
+                        }
                     }
                 }
             }
+            list = block_merge<NW>(list, lists);
         }
-        list = block_merge<NW>(list, lists);
     }
     if (w == 0)
     {
@@ -633,14 +730,13 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
             block_list[lane] = list;
         }
         group.sync();
-        if (part == 0 && w == 0)
+        if (part == 0)
         {
-            for (u32 k = 1; k < cluster; ++k)
-            {
-                sum.join(Sums(*group.map_shared_rank(&block_sums, k)), c);
-                if (a.top)
-                    list = warp_merge(list, group.map_shared_rank(block_list, k)[31 - lane]);
-            }
+            if (w == 0)
+                for (u32 k = 1; k < cluster; ++k)
+                    sum.join(Sums(*group.map_shared_rank(&block_sums, k)), c);
+            if (a.top)  // a warp for each block's list
+                list = block_merge<NW>(w < cluster ? group.map_shared_rank(block_list, w)[lane] : 0, lists);
         }
         group.sync();  // the other blocks' shared memory stays until it has been read
     }
@@ -664,6 +760,7 @@ __global__ void __launch_bounds__(kBackwardBlock) k_logprobs_backward_long(const
     {
         T v[VE];
     };
+    zero_outside<T>(a);
     const u64 r = blockIdx.x / a.slices;
     u64 begin, mask_begin;
     u32 len;
@@ -674,7 +771,7 @@ __global__ void __launch_bounds__(kBackwardBlock) k_logprobs_backward_long(const
     const bool aligned = reinterpret_cast<uintptr_t>(dx) % 16 == 0;
     long long token;
     const Slope slope(a, r, token, len);
-    const u32 token_at_vec = token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u;
+    const u32 own_at = token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u;
     for (u64 i0 = (blockIdx.x % a.slices) * static_cast<u64>(kBackwardBlock * U); i0 < row.count;
          i0 += static_cast<u64>(a.slices) * kBackwardBlock * U)
     {
@@ -706,11 +803,29 @@ __global__ void __launch_bounds__(kBackwardBlock) k_logprobs_backward_long(const
                 row.load_any(j, v);
             Out o;
 #pragma unroll
-            for (int q = 0; q < VE; ++q)
+            for (int q = 0; q < VE; q += 2)
             {
-                const float g = slope(v[q], j * VE + q == token_at_vec);
-                o.v[q] = from_f32<T>(slope.dead || (MASK && v[q] == -kInf) ? 0.f : g);
+                float2 g = slope.of(v[q], v[q + 1]);
+                if (MASK)
+                    g = make_float2(v[q] == -kInf ? 0.f : g.x, v[q + 1] == -kInf ? 0.f : g.y);
+                v[q] = g.x, v[q + 1] = g.y;
             }
+            if (own_at / VE == j)  // seldom: the given token's vector
+            {
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    if (own_at % VE == q && (!MASK || row.mask[own_at]))
+                        v[q] += slope.own;
+            }
+            if (slope.dead)
+            {
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    v[q] = 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < VE; ++q)
+                o.v[q] = from_f32<T>(v[q]);
             T* const to = dx + static_cast<u64>(j) * VE;
             if (whole[k] && aligned)
                 *reinterpret_cast<Out*>(to) = o;

@@ -8,6 +8,7 @@ asynchronous. Statistics and sums are 32-bit whatever the tensors' type (float32
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes as C
 import math
@@ -35,7 +36,8 @@ def _context(t):
 
 
 def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The handle of torch's current stream on t's device (its stream object takes microseconds to make)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 @contextlib.contextmanager
@@ -130,12 +132,11 @@ class _LogProbs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_logprob, grad_entropy, *_):
         logits, tokens, offsets, mask, stats = ctx.saved_tensors  # raises where one was changed in place since
-        g = [None if x is None else x.contiguous() for x in (grad_logprob, grad_entropy)]
-        # of a ragged vector, places may belong to no row
-        make = torch.empty if offsets is None else torch.zeros
-        grad = make(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad_logprob = None if grad_logprob is None else grad_logprob.contiguous()
+        grad_entropy = None if grad_entropy is None else grad_entropy.contiguous()
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         a = ctx.args
-        check(lib().b2_logprobs_backward(_context(logits), C.byref(a), _ptr(g[0]), _ptr(g[1]), grad.data_ptr(),
+        check(lib().b2_logprobs_backward(_context(logits), C.byref(a), _ptr(grad_logprob), _ptr(grad_entropy), grad.data_ptr(),
                                          a.width, _stream(logits)))
         return grad, None, None, None, None, None
 
@@ -344,25 +345,39 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
             raise ValueError(f"adamw_step: 8-bit moments need {name}")
         if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"adamw_step: {name} must be a contiguous {dtype} tensor of {n} elements on {dev}")
-    if int(step) < 1:
+    step = int(step)
+    if step < 1:
         raise ValueError("adamw_step: step counts from 1")
-    kept = []
-    tensors, at = {}, 0  # by (parameter type, gradient type): one launch for each
-    for p, g in zip(params, grads):
-        n = p.numel()
-        if g is not None and n:
-            if p.dtype not in _DTYPE or p.device != dev or not p.is_contiguous():
-                raise ValueError(f"adamw_step: parameters must be contiguous float32, bfloat16 or float16 on {dev}")
-            if g.dtype != p.dtype and g.dtype != torch.float32:
-                raise ValueError("adamw_step: a gradient has its parameter's type or float32")
-            if g.device != dev or g.shape != p.shape:
-                raise ValueError("adamw_step: a gradient has its parameter's shape and device")
-            g = g.contiguous()
-            kept.append(g)
-            tensors.setdefault((_DTYPE[p.dtype], _DTYPE[g.dtype]), []).append((p.data_ptr(), g.data_ptr(), n, at, 0))
-        at += _blocks(n)
+    sizes = [p.numel() for p in params]
+    places, at = [], 0
+    for n in sizes:
+        places.append(at)
+        at += -(-n // BLOCK)
     if at != blocks or elements % BLOCK:
         raise ValueError(f"adamw_step: the moments must hold {at} blocks of {BLOCK} elements, not {elements} elements")
+    if 0 in sizes or any(g is None for g in grads):
+        kept = [i for i, g in enumerate(grads) if g is not None and sizes[i]]
+        live, grads = [params[i] for i in kept], [grads[i] for i in kept]
+        sizes, places = [sizes[i] for i in kept], [places[i] for i in kept]
+    else:
+        live = params
+    if not live:
+        return
+    index = dev.index
+    if {t.get_device() for t in live} | {t.get_device() for t in grads} != {index}:
+        raise ValueError(f"adamw_step: parameters and gradients must be on {dev}")
+    if not all([p.is_contiguous() for p in live]):
+        raise ValueError("adamw_step: parameters must be contiguous")
+    if [g.numel() for g in grads] != sizes:
+        raise ValueError("adamw_step: a gradient has its parameter's shape")
+    if not all([g.is_contiguous() for g in grads]):
+        grads = [g.contiguous() for g in grads]
+    dtypes = [(p.dtype, g.dtype) for p, g in zip(live, grads)]
+    kinds = set(dtypes)
+    for p, g in kinds:
+        if p not in _DTYPE or (g != p and g != torch.float32):
+            raise ValueError("adamw_step: parameters are float32, bfloat16 or float16, a gradient of its parameter's "
+                             "type or float32")
     a = _lib.AdamwArgs()
     a.moment_bits, a.blocks = bits, blocks
     a.exp_avg, a.exp_avg_sq = exp_avg.data_ptr(), exp_avg_sq.data_ptr()
@@ -370,12 +385,16 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
         a.exp_avg_scale, a.exp_avg_sq_scale = exp_avg_scale.data_ptr(), exp_avg_sq_scale.data_ptr()
     a.master = _ptr(master)
     a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = lr, betas, eps, weight_decay
-    a.step, a.seed = int(step), int(seed) & 0xFFFFFFFF
-    for (a.param_dtype, a.grad_dtype), rows in tensors.items():
-        table = (_lib.AdamwTensor * len(rows))(*rows)
-        a.tensors, a.count = C.addressof(table), len(rows)
+    a.step, a.seed = step, int(seed) & 0xFFFFFFFF
+    rows = zip(live, grads, sizes, places)
+    for kind in kinds:  # one launch for each
+        mine = rows if len(kinds) == 1 else [r for r, k in zip(zip(live, grads, sizes, places), dtypes) if k == kind]
+        # the fields of b2_adamw_tensor, as four words
+        table = array.array("Q", [x for p, g, n, b in mine for x in (p.data_ptr(), g.data_ptr(), n, b)])
+        a.tensors, a.count = table.buffer_info()[0], len(table) // 4
+        a.param_dtype, a.grad_dtype = _DTYPE[kind[0]], _DTYPE[kind[1]]
         check(lib().b2_adamw(_context(exp_avg), C.byref(a), _stream(exp_avg)))
-    torch.autograd.graph.increment_version(params)
+    torch.autograd.graph.increment_version(live)
 
 
 class AdamW:
