@@ -772,71 +772,60 @@ __global__ void __launch_bounds__(kBackwardBlock) k_logprobs_backward_long(const
     long long token;
     const Slope slope(a, r, token, len);
     const u32 own_at = token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u;
+    const u32 whole_begin = row.shift ? 1 : 0, whole_end = row.end / VE;
+    auto slopes = [&](float(&v)[VE]) {
+#pragma unroll
+        for (int q = 0; q < VE; q += 2)
+        {
+            float2 g = slope.of(v[q], v[q + 1]);
+            if (MASK)
+                g = make_float2(v[q] == -kInf ? 0.f : g.x, v[q + 1] == -kInf ? 0.f : g.y);
+            v[q] = g.x, v[q + 1] = g.y;
+        }
+    };
     for (u64 i0 = (blockIdx.x % a.slices) * static_cast<u64>(kBackwardBlock * U); i0 < row.count;
          i0 += static_cast<u64>(a.slices) * kBackwardBlock * U)
     {
         const u32 i = static_cast<u32>(i0) + threadIdx.x;
-        uint4 raw[U];
-        u64 allowed[U];
-        bool whole[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k)
+        if (aligned && !slope.dead && i0 >= whole_begin && i0 + kBackwardBlock * U <= whole_end)
         {
-            const u32 j = i + k * kBackwardBlock;
-            whole[k] = j < row.count && row.whole(j);
-            if (whole[k])
+            uint4 raw[U];
+            u64 allowed[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k)
             {
-                raw[k] = row.load_raw(j);
-                allowed[k] = row.load_mask(j);
+                raw[k] = row.load_raw(i + k * kBackwardBlock);
+                allowed[k] = row.load_mask(i + k * kBackwardBlock);
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+            {
+                float v[VE];
+                row.unpack(raw[k], allowed[k], v);
+                slopes(v);
+                Out o;
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    o.v[q] = from_f32<T>(v[q]);
+                *reinterpret_cast<Out*>(dx + static_cast<u64>(i + k * kBackwardBlock) * VE) = o;
             }
         }
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-        {
-            const u32 j = i + k * kBackwardBlock;
-            if (j >= row.count)
-                continue;
-            float v[VE];
-            if (whole[k])
-                row.unpack(raw[k], allowed[k], v);
-            else
+        else
+            for (u32 j = i; j < min(i0 + kBackwardBlock * U, static_cast<u64>(row.count)); j += kBackwardBlock)
+            {
+                float v[VE];
                 row.load_any(j, v);
-            Out o;
-#pragma unroll
-            for (int q = 0; q < VE; q += 2)
-            {
-                float2 g = slope.of(v[q], v[q + 1]);
-                if (MASK)
-                    g = make_float2(v[q] == -kInf ? 0.f : g.x, v[q + 1] == -kInf ? 0.f : g.y);
-                v[q] = g.x, v[q + 1] = g.y;
-            }
-            if (own_at / VE == j)  // seldom: the given token's vector
-            {
-#pragma unroll
-                for (int q = 0; q < VE; ++q)
-                    if (own_at % VE == q && (!MASK || row.mask[own_at]))
-                        v[q] += slope.own;
-            }
-            if (slope.dead)
-            {
-#pragma unroll
-                for (int q = 0; q < VE; ++q)
-                    v[q] = 0.f;
-            }
-#pragma unroll
-            for (int q = 0; q < VE; ++q)
-                o.v[q] = from_f32<T>(v[q]);
-            T* const to = dx + static_cast<u64>(j) * VE;
-            if (whole[k] && aligned)
-                *reinterpret_cast<Out*>(to) = o;
-            else
-            {
+                slopes(v);
 #pragma unroll
                 for (int q = 0; q < VE; ++q)
                     if (j * VE + q >= row.shift && j * VE + q < row.end)
-                        to[q] = o.v[q];
+                        dx[static_cast<u64>(j) * VE + q] = from_f32<T>(slope.dead ? 0.f : v[q]);
             }
-        }
+        // the given token's own part, by the thread that has just written its vector
+        const u32 at = own_at / VE - static_cast<u32>(i0);
+        if (own_at != ~0u && at < kBackwardBlock * U && at % kBackwardBlock == threadIdx.x && !slope.dead &&
+            (!MASK || row.mask[own_at]))
+            dx[own_at] = from_f32<T>(slope.of(to_f32(row.base[own_at]), 0.f).x + slope.own);
     }
 }
 
