@@ -20,6 +20,7 @@ REPO = ROOT.parent
 CSRC = ROOT / "csrc"
 LIB_DIR = ROOT / "lib"
 LIB = LIB_DIR / "libmymyr_b200.so"
+LEARN = LIB_DIR / "_learn.so"  # the learner's operators as a Python module over torch (torch_learn.cpp)
 OBJ_DIR = REPO / "_build" / "mymyr_b200"
 
 CU_SOURCES = ["api.cu", "expand.cu", "brfs.cu", "dbrfs.cu", "comm.cu", "astar.cu", "env.cu", "jit.cu",
@@ -51,6 +52,27 @@ def _stale(out: Path, deps: list[Path]) -> bool:
         return True
     t = out.stat().st_mtime
     return any(d.stat().st_mtime > t for d in deps)
+
+
+def build_learn() -> Path:
+    """The torch module of the learner's operators: host code, linked to the library beside it."""
+    src = CSRC / "torch_learn.cpp"
+    if not _stale(LEARN, [src, REPO / "include" / "mymyr_b200.h"]):
+        return LEARN
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    inc = [REPO / "include", *include_paths(), "/usr/local/cuda/include", sysconfig.get_paths()["include"]]
+    tmp = LEARN.with_suffix(".so.tmp")
+    _run(["g++", "-std=c++20", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
+          "-DTORCH_EXTENSION_NAME=_learn", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[f"-isystem{p}" for p in inc], str(src), "-o", str(tmp), f"-L{LIB_DIR}", "-l:libmymyr_b200.so",
+          "-Wl,-rpath,$ORIGIN", *[f"-L{p}" for p in library_paths()], "-ltorch_python", "-ltorch", "-ltorch_cpu",
+          "-lc10_cuda", "-lc10"])
+    tmp.replace(LEARN)
+    return LEARN
 
 
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
@@ -93,6 +115,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         tmp = LIB.with_suffix(".so.tmp")
         _run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs), "-ldl"])
         tmp.replace(LIB)
+    build_learn()
     if verbose:
         print(f"built {LIB}")
     return LIB
