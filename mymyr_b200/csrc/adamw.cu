@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 namespace b2
 {
@@ -116,10 +117,24 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8])
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-__device__ __forceinline__ float sqrt_approx(float x)
+/// Fast square root and reciprocal of normal numbers (2 units in the last place).
+__device__ __forceinline__ float sqrt_fast(float x)
 {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+/// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_magnitude(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
     return r;
 }
 
@@ -135,29 +150,30 @@ __device__ __forceinline__ float scale_of(u32 largest)
 __device__ __forceinline__ float inverse_power(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
 
 /// The warp's largest finite magnitude, as bits. Magnitudes order as their bits do; where an infinity or a NaN leads, the
-/// others are looked through again without it.
+/// others are looked through again without it, and the result has its sign bit set.
 __device__ __forceinline__ u32 largest_of(const float (&x)[8])
 {
-    u32 top = 0;
+    float most = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-        top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
-    u32 all = __reduce_max_sync(~0u, top);
+        most = max_magnitude(most, x[k]);
+    u32 all = __reduce_max_sync(~0u, __float_as_uint(most));
     if (all >= kInfBits)
     {
-        top = 0;
+        u32 top = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
         {
             const u32 u = __float_as_uint(x[k]) & 0x7FFFFFFFu;
             top = max(top, u < kInfBits ? u : 0u);
         }
-        all = __reduce_max_sync(~0u, top) | 0x80000000u;  // the sign: some were left out
+        all = __reduce_max_sync(~0u, top) | 0x80000000u;
     }
     return all;
 }
 
-/// A warp for each block of 256 elements, lane l with the eight from 8 l on.
+/// A warp for each block of 256 elements, lane l with the eight from 8 l on; `run` blocks in a row, so that the pointers
+/// just advance between them.
 ///
 /// Bound by HBM in 32 bits (28 bytes for an element: parameter, gradient and moments read, all but the gradient written)
 /// and nearly as much by instruction issue in 8 bits (10 bytes). One pass: everything of an element is in registers
@@ -166,10 +182,16 @@ __device__ __forceinline__ u32 largest_of(const float (&x)[8])
 /// then are those of the formula as written, on any machine.
 template<class P, class G, int BITS, bool MASTER, u32 N>
 __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
-                                                       u32 key)
+                                                       u32 key, u32 run)
 {
+    using M = std::conditional_t<BITS == 8, uint8_t, float>;
     const u32 lane = threadIdx.x & 31, i0 = lane * 8;
-    u32 b = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const u64 warp = static_cast<u64>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const u64 from = warp * run;
+    if (from >= t.blocks)
+        return;
+    u32 b = static_cast<u32>(from);
+    const u32 stop = static_cast<u32>(min(from + run, static_cast<u64>(t.blocks)));
     u32 entry = 0;
     {
         u32 hi = t.count;
@@ -179,20 +201,36 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
             (t.e[mid].begin <= b ? entry : hi) = mid;
         }
     }
-    for (; b < t.blocks; b += gridDim.x * kWarps)
+    const Two b1(h.b1, h.b1), a1(h.a1, h.a1), b2(h.b2, h.b2), a2(h.a2, h.a2);
+    P* p = nullptr;
+    const G* g = nullptr;
+    M *m_at = nullptr, *v_at = nullptr;
+    float* master = nullptr;
+    u64 left = 0;  // elements of the tensor from this block on
+    u32 block = 0, next_entry = b;
+    bool aligned = false;
+    for (; b < stop; ++b)
     {
-        while (entry + 1 < t.count && t.e[entry + 1].begin <= b)
-            ++entry;
-        const Entry& e = t.e[entry];
-        const u64 first = static_cast<u64>(b - e.begin) * kMoment;  // in the tensor
-        const u32 block = e.block + (b - e.begin);
-        const u64 at = static_cast<u64>(block) * kMoment + i0;  // in the moments, which hold whole blocks
-        const u32 n = static_cast<u32>(e.n - first < kMoment ? e.n - first : kMoment);
-        P* const p = static_cast<P*>(e.p) + first + i0;
-        const G* const g = static_cast<const G*>(e.g) + first + i0;
+        if (b >= next_entry)
+        {
+            while (entry + 1 < t.count && t.e[entry + 1].begin <= b)
+                ++entry;
+            const Entry& e = t.e[entry];
+            next_entry = entry + 1 < t.count ? t.e[entry + 1].begin : ~0u;
+            block = e.block + (b - e.begin);
+            const u64 first = static_cast<u64>(b - e.begin) * kMoment;  // in the tensor
+            const u64 at = static_cast<u64>(block) * kMoment + i0;      // in the moments, which hold whole blocks
+            left = e.n - first;
+            p = static_cast<P*>(e.p) + first + i0;
+            g = static_cast<const G*>(e.g) + first + i0;
+            m_at = static_cast<M*>(s.m) + at;
+            v_at = static_cast<M*>(s.v) + at;
+            master = s.master + at;
+            aligned = !(reinterpret_cast<uintptr_t>(e.p) & kAlign8<P>) && !(reinterpret_cast<uintptr_t>(e.g) & kAlign8<G>);
+        }
         // a tensor's last block, and tensors that start off a vector's boundary, go element by element
-        const bool whole = n == kMoment && !(reinterpret_cast<uintptr_t>(e.p) & kAlign8<P>) &&
-                           !(reinterpret_cast<uintptr_t>(e.g) & kAlign8<G>);
+        const u32 n = static_cast<u32>(min(left, static_cast<u64>(kMoment)));
+        const bool whole = aligned && n == kMoment;
         float gi[8], now[8], m[8], v[8], r[8];
         if (whole)
         {
@@ -211,11 +249,11 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
             }
         }
         if constexpr (MASTER)
-            load8(s.master + at, now);
+            load8(master, now);
         if constexpr (BITS == 8)
         {
-            decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.m) + at), m);
-            decode8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.v) + at), r);
+            decode8(*reinterpret_cast<const uint2*>(m_at), m);
+            decode8(*reinterpret_cast<const uint2*>(v_at), r);
             const float ms = s.m_scale[block], vs = s.v_scale[block];
             const Two ms2(ms, ms), vs2(vs, vs);
 #pragma unroll
@@ -229,10 +267,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
         }
         else
         {
-            load8(static_cast<const float*>(s.m) + at, m);
-            load8(static_cast<const float*>(s.v) + at, v);
+            load8(m_at, m);
+            load8(v_at, v);
         }
-        const Two b1(h.b1, h.b1), a1(h.a1, h.a1), b2(h.b2, h.b2), a2(h.a2, h.a2);
 #pragma unroll
         for (int k = 0; k < 8; k += 2)
         {
@@ -244,11 +281,11 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
 #pragma unroll
         for (int k = 0; k < 8; ++k)
         {
-            r[k] = sqrt_approx(v[k]);
-            now[k] = now[k] * h.decay - __fdividef(m[k] * h.rate, r[k] * h.correct + h.eps);
+            r[k] = sqrt_fast(fmaxf(v[k], 0x1p-126f));  // normal numbers; the divisor is not zero
+            now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(r[k] * h.correct + h.eps));
         }
         if constexpr (MASTER)
-            store8(s.master + at, now);
+            store8(master, now);
         if (whole)
             store8(p, now);
         else
@@ -260,8 +297,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
         }
         if constexpr (BITS == 32)
         {
-            store8(static_cast<float*>(s.m) + at, m);
-            store8(static_cast<float*>(s.v) + at, v);
+            store8(m_at, m);
+            store8(v_at, v);
         }
         else
         {
@@ -275,17 +312,18 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     m[k] = m[k] - m[k] == 0.f ? m[k] : nanf("");
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + at) = encode8(m);
+            *reinterpret_cast<uint2*>(m_at) = encode8(m);
             top = largest_of(v);
             bad = top >> 31;
             // the square root of the largest is the largest square root
             const float vs = scale_of(__float_as_uint(__fsqrt_rn(__uint_as_float(top & 0x7FFFFFFFu))));
             const float vi = inverse_power(vs);
+            const u32 pair = block * (kMoment / 2) + i0 / 2;  // of the element among all, modulo 2^32
             float code[8];
 #pragma unroll
             for (int k = 0; k < 8; k += 2)
             {
-                const u32 bits = mix((static_cast<u32>(at >> 1) + k / 2) ^ key);
+                const u32 bits = mix((pair + k / 2) ^ key);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                 {
@@ -308,13 +346,15 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     code[k] = v[k] - v[k] == 0.f ? code[k] : nanf("");
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + at) = encode8(code);
+            *reinterpret_cast<uint2*>(v_at) = encode8(code);
             if (lane == 0)
             {
                 s.m_scale[block] = ms;
                 s.v_scale[block] = vs;
             }
         }
+        p += kMoment, g += kMoment, m_at += kMoment, v_at += kMoment, master += kMoment;
+        left -= n, ++block;
     }
 }
 
@@ -333,8 +373,11 @@ void launch(const b2_ctx& ctx, const b2_adamw_args& a, u32 first, u32 count, con
     t.blocks = static_cast<u32>(blocks);
     const u32 key = mix(mix(a.seed) ^ static_cast<u32>(a.step));
     const Moments s{a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.master};
-    const unsigned grid = grid_for(blocks, kWarps, static_cast<unsigned>(ctx.sms) * 16);
-    k_adamw<P, G, BITS, MASTER, N><<<grid, kWarps * 32, 0, st>>>(t, s, h, key);
+    // runs of up to eight blocks, while every warp that the device holds has one
+    const u32 run = static_cast<u32>(std::min<u64>(8, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 32))));
+    const u64 per = static_cast<u64>(kWarps) * run;
+    k_adamw<P, G, BITS, MASTER, N>
+        <<<static_cast<unsigned>((blocks + per - 1) / per), kWarps * 32, 0, st>>>(t, s, h, key, run);
     B2_CUDA(cudaGetLastError());
 }
 
