@@ -149,14 +149,10 @@ __device__ __forceinline__ float scale_of(u32 largest)
 /// 1 / scale, exactly.
 __device__ __forceinline__ float inverse_power(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
 
-/// The warp's largest finite magnitude, as bits. Magnitudes order as their bits do; where an infinity or a NaN leads, the
-/// others are looked through again without it, and the result has its sign bit set.
-__device__ __forceinline__ u32 largest_of(const float (&x)[8])
+/// The warp's largest finite magnitude, as bits, from each lane's largest. Magnitudes order as their bits do; where an
+/// infinity or a NaN leads, the lanes' values are looked through again without it, and the result has its sign bit set.
+__device__ __forceinline__ u32 largest_of(float most, const float (&x)[8])
 {
-    float most = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        most = max_magnitude(most, x[k]);
     u32 all = __reduce_max_sync(~0u, __float_as_uint(most));
     if (all >= kInfBits)
     {
@@ -172,6 +168,14 @@ __device__ __forceinline__ u32 largest_of(const float (&x)[8])
     return all;
 }
 
+/// 1 if x is above 2^-63, else 0, for x of at least 2^-63.
+__device__ __forceinline__ float above_least(float x)
+{
+    float r;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(0x1p87f), "f"(-0x1p24f));
+    return r;
+}
+
 /// A warp for each block of 256 elements, lane l with the eight from 8 l on; `run` blocks in a row, so that the pointers
 /// just advance between them.
 ///
@@ -181,7 +185,7 @@ __device__ __forceinline__ u32 largest_of(const float (&x)[8])
 /// the moments' arithmetic runs in pairs. Averages are separate multiplications and additions (not fused): the scales
 /// then are those of the formula as written, on any machine.
 template<class P, class G, int BITS, bool MASTER, u32 N>
-__global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
+__global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
                                                        u32 key, u32 run)
 {
     using M = std::conditional_t<BITS == 8, uint8_t, float>;
@@ -278,11 +282,20 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
             const float2 y = (Two(v[k], v[k + 1]) * b2 + g2 * g2 * a2).get();
             m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
         }
+        float m_most = 0.f, v_most = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
         {
-            r[k] = sqrt_fast(fmaxf(v[k], 0x1p-126f));  // normal numbers; the divisor is not zero
+            // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
+            float floor;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
+            r[k] = sqrt_fast(floor);
             now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(r[k] * h.correct + h.eps));
+            if constexpr (BITS == 8)
+            {
+                m_most = max_magnitude(m_most, m[k]);
+                v_most = max_magnitude(v_most, v[k]);
+            }
         }
         if constexpr (MASTER)
             store8(master, now);
@@ -302,7 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
         }
         else
         {
-            u32 top = largest_of(m);
+            u32 top = largest_of(m_most, m);
             bool bad = top >> 31;
             const float ms = scale_of(top), mi = inverse_power(ms);
 #pragma unroll
@@ -313,11 +326,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
                 for (int k = 0; k < 8; ++k)
                     m[k] = m[k] - m[k] == 0.f ? m[k] : nanf("");
             *reinterpret_cast<uint2*>(m_at) = encode8(m);
-            top = largest_of(v);
-            bad = top >> 31;
             // the square root of the largest is the largest square root
-            const float vs = scale_of(__float_as_uint(__fsqrt_rn(__uint_as_float(top & 0x7FFFFFFFu))));
-            const float vi = inverse_power(vs);
+            top = __reduce_max_sync(~0u, __float_as_uint(v_most));
+            bad = top >= kInfBits;
+            top = bad ? largest_of(__uint_as_float(top), r) : __float_as_uint(__fsqrt_rn(__uint_as_float(top)));
+            const float vs = scale_of(top);
+            const u32 vs_exponent = __float_as_uint(vs) - (127u << 23);
             const u32 pair = block * (kMoment / 2) + i0 / 2;  // of the element among all, modulo 2^32
             float code[8];
 #pragma unroll
@@ -327,25 +341,23 @@ __global__ void __launch_bounds__(kWarps * 32) k_adamw(const __grid_constant__ T
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                 {
-                    // (16 bits + 1/2) / 2^16, by way of a number in [1, 2)
-                    const u32 part = j ? bits >> 16 : bits & 0xFFFFu;
-                    const float u = __uint_as_float(0x3F800040u | part << 7) - 1.f;
-                    // x / unit is in [8, 16), or below 8 among the smallest codes; its floor, by way of 2^23
-                    const float x = r[k + j] * vi;
-                    const u32 ex = max(__float_as_uint(x) & kInfBits, 121u << 23);
-                    const float q = x * __uint_as_float((257u << 23) - ex);
+                    // u = (16 bits + 1/2) / 2^16 as the number 1 + u
+                    const u32 part = j ? bits >> 9 : bits << 7;
+                    const float u1 = __uint_as_float(0x3F800040u | (part & 0x7FFF80u));
+                    // r / (unit scale) is in [8, 16), or below 8 among the smallest codes; its floor, by way of 2^23
+                    const u32 ex = max(__float_as_uint(r[k + j]) & kInfBits, (121u << 23) + vs_exponent);
+                    const float q = r[k + j] * __uint_as_float((257u << 23) - ex);
                     const float low = __fadd_rd(q, 0x1p23f) - 0x1p23f;
                     // up with the probability that keeps the square's mean: (q^2 - low^2) / ((low + 1)^2 - low^2)
-                    const float edge = fmaf(u, fmaf(2.f, low, 1.f), low * low);
-                    float c = (q * q > edge ? low + 1.f : low) * __uint_as_float(ex - (3u << 23));
-                    c = v[k + j] > 0.f ? fmaxf(c, 0x1p-9f) : 0.f;
-                    code[k + j] = c;
+                    const float step = fmaf(2.f, low, 1.f), edge = fmaf(u1, step, fmaf(low, low, -step));
+                    const float up = q * q > edge ? low + 1.f : low;
+                    code[k + j] = fmaxf(up, above_least(r[k + j])) * __uint_as_float(ex - (3u << 23) - vs_exponent);
                 }
             }
             if (bad)
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    code[k] = v[k] - v[k] == 0.f ? code[k] : nanf("");
+                    code[k] = r[k] - r[k] == 0.f ? code[k] : nanf("");
             *reinterpret_cast<uint2*>(v_at) = encode8(code);
             if (lane == 0)
             {
@@ -373,8 +385,8 @@ void launch(const b2_ctx& ctx, const b2_adamw_args& a, u32 first, u32 count, con
     t.blocks = static_cast<u32>(blocks);
     const u32 key = mix(mix(a.seed) ^ static_cast<u32>(a.step));
     const Moments s{a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.master};
-    // runs of up to eight blocks, while every warp that the device holds has one
-    const u32 run = static_cast<u32>(std::min<u64>(8, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 32))));
+    // runs of up to eight blocks, while the warps that the device holds have four each
+    const u32 run = static_cast<u32>(std::min<u64>(8, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 128))));
     const u64 per = static_cast<u64>(kWarps) * run;
     k_adamw<P, G, BITS, MASTER, N>
         <<<static_cast<unsigned>((blocks + per - 1) / per), kWarps * 32, 0, st>>>(t, s, h, key, run);
