@@ -50,16 +50,16 @@ struct Zeros
 };
 __device__ __forceinline__ void write_zeros(const Zeros& z, u64 thread, u64 threads)
 {
-    const u64 head = min(z.bytes, static_cast<u64>(-reinterpret_cast<uintptr_t>(z.p) & 15));
+    const u64 head = min(z.bytes, static_cast<u64>(-reinterpret_cast<uintptr_t>(z.p) & 31));
     char* const p = static_cast<char*>(z.p);
-    uint4* const v = reinterpret_cast<uint4*>(p + head);
-    const u64 n = (z.bytes - head) / 16;
+    char* const v = p + head;
+    const u64 n = (z.bytes - head) / 32;
     for (u64 i = thread; i < n; i += threads)
-        v[i] = make_uint4(0, 0, 0, 0);
-    const u64 tail = head + n * 16;
+        asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"l"(v + i * 32), "r"(0) : "memory");
+    const u64 tail = head + n * 32;
     if (thread < head)
         p[thread] = 0;
-    if (tail + thread < z.bytes && thread < 16)
+    if (thread < z.bytes - tail)
         p[tail + thread] = 0;
 }
 
@@ -136,7 +136,8 @@ constexpr size_t cluster_bytes(u32 share)
 /// of a table of 1,024 columns; as separate launches of count, scan and scatter kernels it took 44 us before them.
 __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const Tokens in, u32 n, u32 share, u32 passes, u32 bits,
                                                                   u32* __restrict__ keys, u32* __restrict__ places,
-                                                                  u32* __restrict__ held_count, const Zeros zeros)
+                                                                  u32* __restrict__ held_count, u32* __restrict__ joins,
+                                                                  u32* __restrict__ long_joins, const Zeros zeros)
 {
     const u32 t = threadIdx.x, lane = t & 31, w = t >> 5;
     if (blockIdx.x >= kClusterBlocks)
@@ -239,7 +240,10 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const Tokens i
         cluster.sync();
     }
     if (q == 0 && t == 0)
+    {
         *held_count = total;
+        joins[0] = long_joins[0] = 0;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- sort over the device
@@ -282,7 +286,8 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_count(const Pass in, u32* _
         return;
     }
     __shared__ u32 bins[kBins];
-    bins[threadIdx.x] = 0;
+    if (threadIdx.x < kBins)
+        bins[threadIdx.x] = 0;
     __syncthreads();
     const u32 base = blockIdx.x * kSortTile, size = in.size();
 #pragma unroll
@@ -293,16 +298,17 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_count(const Pass in, u32* _
             atomicAdd(&bins[in.digit(key)], 1u);
     }
     __syncthreads();
-    counts[threadIdx.x * in.tiles + blockIdx.x] = bins[threadIdx.x];
+    if (threadIdx.x < 1u << in.bits)
+        counts[threadIdx.x * in.tiles + blockIdx.x] = bins[threadIdx.x];
 }
 
 /// A block for each digit: its tiles' counts become their exclusive sums, its total goes to totals[digit].
-__global__ void __launch_bounds__(kSortBlock) k_sort_scan(u32* __restrict__ counts, u32 tiles, u32* __restrict__ totals)
+__global__ void __launch_bounds__(kBins) k_sort_scan(u32* __restrict__ counts, u32 tiles, u32* __restrict__ totals)
 {
     __shared__ u32 tmp[kBins / 32];
     u32* row = counts + static_cast<u64>(blockIdx.x) * tiles;
     u32 carry = 0;
-    for (u32 t = 0; t < tiles; t += kSortBlock)
+    for (u32 t = 0; t < tiles; t += kBins)
     {
         const u32 i = t + threadIdx.x;
         const u32 v = i < tiles ? row[i] : 0;
@@ -319,7 +325,8 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scan(u32* __restrict__ coun
 /// Each key to its digit's place, equal digits in the order they came in; the number of keys to held_count.
 __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Pass in, const u32* __restrict__ counts,
                                                              const u32* __restrict__ totals, u32* __restrict__ keys,
-                                                             u32* __restrict__ places, u32* __restrict__ held_count)
+                                                             u32* __restrict__ places, u32* __restrict__ held_count,
+                                                             u32* __restrict__ joins, u32* __restrict__ long_joins)
 {
     __shared__ u32 at[kSortBlock / 32][kBins];
     __shared__ u32 tmp[kBins / 32];
@@ -341,16 +348,22 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Pass in, cons
     for (u32 k = 0; k < kSortRounds; ++k)
         rank[k] = warp_rank(in.digit(key[k]), held >> k & 1, in.bits, at[w]);
     const u32 d = threadIdx.x;
+    const bool digit = d < 1u << in.bits;
+    const u32 before = digit ? counts[d * in.tiles + blockIdx.x] : 0;
     u32 all;
-    u32 run = digits_exclusive(totals[d], tmp, &all) + counts[d * in.tiles + blockIdx.x];
-    for (u32 i = 0; i < kSortBlock / 32; ++i)
-    {
-        const u32 c = at[i][d];
-        at[i][d] = run;
-        run += c;
-    }
+    u32 run = digits_exclusive(digit ? totals[d] : 0, tmp, &all) + before;
+    if (digit)
+        for (u32 i = 0; i < kSortBlock / 32; ++i)
+        {
+            const u32 c = at[i][d];
+            at[i][d] = run;
+            run += c;
+        }
     if (held_count && blockIdx.x == 0 && threadIdx.x == 0)
+    {
         *held_count = all;
+        joins[0] = long_joins[0] = 0;
+    }
     __syncthreads();
 #pragma unroll
     for (u32 k = 0; k < kSortRounds; ++k)
@@ -374,6 +387,8 @@ struct Segments
     float scale;
     u64 width, grad_stride;
     float* partial;  // [chunks, 2, width]: of the token that comes into the chunk, of the one that goes on after it
+    u32* joins;       // the number of chunks out of which a token goes on that did not come into them, and these chunks
+    u32* long_joins;  // of them, those whose token comes into many chunks
 };
 
 template<class T, int VE>
@@ -386,11 +401,11 @@ __device__ __forceinline__ void store_scaled(T* to, const float* sum, float scal
     *reinterpret_cast<Vec<T, VE>*>(to) = o;
 }
 
-/// A thread for each chunk and vector of columns; eight gradient rows are under way at a time.
+/// A thread for each chunk and vector of columns; four gradient rows are under way at a time.
 template<class T, int VE>
 __global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* __restrict__ grad, T* __restrict__ out)
 {
-    constexpr u32 U = 8;
+    constexpr u32 U = 4;
     const u64 id = static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x;
     const u64 items = static_cast<u64>(a.chunks) * a.columns;
     if (id >= items)
@@ -448,91 +463,124 @@ __global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* 
                 sum[j] += to_f32(g[k].v[j]);
         }
     }
-    flush(end < n && a.keys[end] == current);
+    const bool goes_on = end < n && a.keys[end] == current;
+    flush(goes_on);
+    if (goes_on && !comes_in && offset == 0)  // in any order: each is joined by itself
+        a.joins[1 + atomicAdd(a.joins, 1u)] = c;
 }
 
-constexpr u32 kJoinColumns = 128;
+constexpr u32 kJoinColumns = 128, kJoinShort = 16;
 
-/// A block for each chunk out of which a token goes on that did not come into it, and 128 columns: its warps take the
-/// partial sums of every eighth chunk, and their sums are added in the warps' order.
+/// Joins the partial sums of each token that crosses a few chunks, a warp for a token and 128 columns; a token of more
+/// chunks goes to the list of the long ones.
 template<class T>
-__global__ void __launch_bounds__(256) k_segment_join(const Segments a, T* __restrict__ out)
+__global__ void __launch_bounds__(256) k_segment_join(const Segments a, T* __restrict__ out, u32 slices)
 {
-    __shared__ float sums[8][kJoinColumns];
-    const u32 c = blockIdx.x, n = *a.count;
-    const u64 begin = static_cast<u64>(c) * a.chunk, end = begin + a.chunk;
-    if (end >= n)
-        return;
-    const u32 key = a.keys[end];
-    if (a.keys[end - 1] != key || (begin && a.keys[begin - 1] == key))
-        return;
-    u32 more = 1;  // chunks that the token comes into
-    for (;;)
+    const u32 n = *a.count, lane = threadIdx.x & 31;
+    const u64 items = static_cast<u64>(a.joins[0]) * slices;
+    for (u64 item = (static_cast<u64>(blockIdx.x) * 256 + threadIdx.x) / 32; item < items; item += gridDim.x * 8ull)
     {
-        const u64 first = (static_cast<u64>(c) + 1 + more + threadIdx.x) * a.chunk;
-        const u32 got = __syncthreads_count(first < n && a.keys[first] == key);
-        more += got;
-        if (got < blockDim.x)
-            break;
-    }
-    const u32 lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const u64 column = static_cast<u64>(blockIdx.y) * kJoinColumns + lane;
-    float sum[kJoinColumns / 32] = {};
+        const u32 c = a.joins[1 + item / slices], slice = static_cast<u32>(item % slices);
+        const u32 key = a.keys[static_cast<u64>(c + 1) * a.chunk];
+        const u64 first = (static_cast<u64>(c) + 1 + lane) * a.chunk;
+        const u32 span = __popc(__ballot_sync(~0u, first < n && a.keys[first] == key));  // chunks that it comes into
+        if (span > kJoinShort)
+        {
+            if (slice == 0 && lane == 0)
+                a.long_joins[1 + atomicAdd(a.long_joins, 1u)] = c;
+            continue;
+        }
+        const u64 column = static_cast<u64>(slice) * kJoinColumns + lane;
+        const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
+        float sum[kJoinColumns / 32] = {};
 #pragma unroll 4
-    for (u32 i = w; i <= more; i += 8)
-    {
-        // the first partial sum is of the token that goes on, the others of the one that comes in
-        const float* from = a.partial + ((static_cast<u64>(c) + i) * 2 + (i == 0)) * a.width + column;
+        for (u32 i = 0; i <= span; ++i)
+        {
+            // the first partial sum is of the token that goes on, the others of the one that comes in
+#pragma unroll
+            for (u32 k = 0; k < kJoinColumns / 32; ++k)
+                if (column + k * 32 < a.width)
+                    sum[k] += from[(static_cast<u64>(i) * 2 + (i == 0)) * a.width + k * 32];
+        }
 #pragma unroll
         for (u32 k = 0; k < kJoinColumns / 32; ++k)
             if (column + k * 32 < a.width)
-                sum[k] += from[k * 32];
+                out[key * a.width + column + k * 32] = from_f32<T>(sum[k] * a.scale);
     }
-#pragma unroll
-    for (u32 k = 0; k < kJoinColumns / 32; ++k)
-        sums[w][k * 32 + lane] = sum[k];
-    __syncthreads();
-    const u64 col = static_cast<u64>(blockIdx.y) * kJoinColumns + threadIdx.x;
-    if (threadIdx.x < kJoinColumns && col < a.width)
+}
+
+/// Those of many chunks, a block for a token and `lanes` columns (a power of two up to 32): 256 / lanes rows of threads
+/// over the chunks, whose sums are added as a tree.
+template<class T>
+__global__ void __launch_bounds__(256) k_segment_join_long(const Segments a, T* __restrict__ out, u32 lanes, u32 slices)
+{
+    __shared__ float sums[256];
+    const u32 n = *a.count, rows = 256 / lanes, row = threadIdx.x / lanes;
+    const u64 items = static_cast<u64>(a.long_joins[0]) * slices;
+    for (u64 item = blockIdx.x; item < items; item += gridDim.x)
     {
-        float all = 0;
-        for (u32 i = 0; i < 8; ++i)
-            all += sums[i][threadIdx.x];
-        out[key * a.width + col] = from_f32<T>(all * a.scale);
+        const u32 c = a.long_joins[1 + item / slices], key = a.keys[static_cast<u64>(c + 1) * a.chunk];
+        const u64 column = item % slices * lanes + (threadIdx.x & (lanes - 1));
+        u32 more = 1;
+        for (;;)
+        {
+            const u64 first = (static_cast<u64>(c) + 1 + more + threadIdx.x) * a.chunk;
+            const u32 got = __syncthreads_count(first < n && a.keys[first] == key);
+            more += got;
+            if (got < blockDim.x)
+                break;
+        }
+        float sum = 0.f;
+        if (column < a.width)
+        {
+            const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
+#pragma unroll 8
+            for (u32 i = row; i <= more; i += rows)
+                sum += from[(static_cast<u64>(i) * 2 + (i == 0)) * a.width];
+        }
+        sums[threadIdx.x] = sum;
+        __syncthreads();
+        for (u32 half = rows / 2; half; half /= 2)
+        {
+            if (row < half)
+                sums[threadIdx.x] += sums[threadIdx.x + half * lanes];
+            __syncthreads();
+        }
+        if (row == 0 && column < a.width)
+            out[key * a.width + column] = from_f32<T>(sums[threadIdx.x] * a.scale);
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------------------------------------- lookup
 
-constexpr u32 kLookupRows = 4;
-
-/// A thread for each vector of columns and four rows.
-template<class T, int VE>
+/// A thread for each vector of columns and ROWS rows.
+template<class T, int VE, u32 ROWS>
 __global__ void __launch_bounds__(256) k_lookup(const b2_embedding_args a, const T* __restrict__ weight, u64 stride,
                                                 T* __restrict__ rows, u32 columns)
 {
     const u64 id = static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const u64 groups = (a.count + kLookupRows - 1) / kLookupRows, items = groups * columns;
+    const u64 groups = (a.count + ROWS - 1) / ROWS, items = groups * columns;
     if (id >= items)
         return;
     const u64 group = items >> 32 ? id / columns : static_cast<u32>(id) / columns;
     const u64 offset = (id - group * columns) * VE;
-    long long t[kLookupRows];
-    Vec<T, VE> x[kLookupRows];
+    long long t[ROWS];
+    Vec<T, VE> x[ROWS];
 #pragma unroll
-    for (u32 k = 0; k < kLookupRows; ++k)
+    for (u32 k = 0; k < ROWS; ++k)
     {
-        const u64 r = group * kLookupRows + k;
+        const u64 r = group * ROWS + k;
         t[k] = r < a.count ? token_at(a.tokens, a.token_bits, r) : -1;
     }
 #pragma unroll
-    for (u32 k = 0; k < kLookupRows; ++k)
+    for (u32 k = 0; k < ROWS; ++k)
         if (t[k] >= 0 && t[k] < static_cast<long long>(a.vocabulary))
             x[k] = *reinterpret_cast<const Vec<T, VE>*>(weight + t[k] * stride + offset);
 #pragma unroll
-    for (u32 k = 0; k < kLookupRows; ++k)
+    for (u32 k = 0; k < ROWS; ++k)
     {
-        const u64 r = group * kLookupRows + k;
+        const u64 r = group * ROWS + k;
         const bool in = t[k] >= 0 && t[k] < static_cast<long long>(a.vocabulary);
 #pragma unroll
         for (int j = 0; j < VE; ++j)
@@ -573,7 +621,7 @@ struct Plan
 {
     u32 n, passes, bits, tiles, chunk, chunks;
     bool cluster;
-    size_t keys[2], places[2], counts, totals, held, partial, bytes;
+    size_t keys[2], places[2], counts, totals, held, joins, long_joins, partial, bytes;
 };
 
 Plan plan_of(const b2_embedding_args& a)
@@ -587,11 +635,13 @@ Plan plan_of(const b2_embedding_args& a)
     p.bits = (bits + p.passes - 1) / p.passes;
     p.cluster = p.n <= kClusterMost;
     p.tiles = (p.n + kSortTile - 1) / kSortTile;
-    // chunks as short as leaves a thread for each of 1,024 in an SM: long enough to keep partial sums few, short enough
+    // chunks as short as leaves a thread for each of 2,048 in an SM: long enough to keep partial sums few, short enough
     // to fill the device (columns counted as vectors of 16 bytes)
     const u64 columns = std::max<u64>(1, a.width * size_of(a.dtype) / 16);
-    const u64 even = a.count * columns / (148 * 1024);
-    p.chunk = static_cast<u32>(std::min<u64>(256, std::max<u64>(8, (even + 7) / 8 * 8)));
+    const u64 even = a.count * columns / (148 * 2048);
+    // at most 16,384 of them: a frequent token's partial sums are joined one after the other
+    const u64 least = std::max<u64>(8, a.count >> 14);
+    p.chunk = static_cast<u32>((std::max(least, std::min<u64>(256, even)) + 7) / 8 * 8);
     p.chunks = (p.n + p.chunk - 1) / p.chunk;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -611,6 +661,8 @@ Plan plan_of(const b2_embedding_args& a)
         p.totals = take(kBins * 4);
     }
     p.held = take(4);
+    p.joins = take((static_cast<size_t>(p.chunks) + 1) * 4);
+    p.long_joins = take((static_cast<size_t>(p.chunks) + 1) * 4);
     p.partial = take(static_cast<size_t>(p.chunks) * 2 * a.width * 4);
     p.bytes = at;
     return p;
@@ -623,8 +675,10 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
 {
     auto words = [&](size_t at) { return reinterpret_cast<u32*>(ws + at); };
     const Tokens tokens{a.tokens, a.token_bits, static_cast<u32>(a.vocabulary)};
-    const u64 vectors = zeros.bytes / 16 + 1;
+    const u64 vectors = zeros.bytes / 32 + 1;
     s.count = words(p.held);
+    s.joins = words(p.joins);
+    s.long_joins = words(p.long_joins);
     if (p.cluster)
     {
         const u32 share = std::max(1u, (p.n + kClusterBlocks * kClusterThreads - 1) / (kClusterBlocks * kClusterThreads)) *
@@ -635,8 +689,8 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
             B2_CUDA(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(cluster_bytes(kClusterThreads * kClusterRounds))));
         });
-        // a block of zeros for each SM that the sort leaves, while there is a vector for each thread
-        const u64 most = static_cast<u64>(ctx.sms) / kClusterBlocks * kClusterBlocks - kClusterBlocks;
+        // up to four blocks of zeros for each SM, while there is a vector for each thread
+        const u64 most = static_cast<u64>(ctx.sms) / kClusterBlocks * kClusterBlocks * 4 - kClusterBlocks;
         const u64 want = (vectors + kClusterThreads - 1) / kClusterThreads;
         const u64 blocks = (std::min(most, want) + kClusterBlocks - 1) / kClusterBlocks * kClusterBlocks;
         cudaLaunchConfig_t cfg{};
@@ -653,7 +707,7 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
         s.keys = words(p.keys[0]);
         s.places = words(p.places[0]);
         B2_CUDA(cudaLaunchKernelEx(&cfg, k_sort_cluster, tokens, p.n, share, p.passes, p.bits, words(p.keys[0]),
-                                   words(p.places[0]), words(p.held), zeros));
+                                   words(p.places[0]), words(p.held), words(p.joins), words(p.long_joins), zeros));
         return;
     }
     Pass in{tokens, nullptr, nullptr, nullptr, p.n, 0, p.bits, p.tiles};
@@ -664,9 +718,10 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
         u32* const places = words(p.places[i & 1]);
         const unsigned extra = i == 0 ? grid_for(vectors, kSortBlock, static_cast<unsigned>(ctx.sms) * 8) : 0;
         k_sort_count<<<p.tiles + extra, kSortBlock, 0, st>>>(in, words(p.counts), zeros);
-        k_sort_scan<<<kBins, kSortBlock, 0, st>>>(words(p.counts), p.tiles, words(p.totals));
+        k_sort_scan<<<1u << p.bits, kBins, 0, st>>>(words(p.counts), p.tiles, words(p.totals));
         k_sort_scatter<<<p.tiles, kSortBlock, 0, st>>>(in, words(p.counts), words(p.totals), keys, places,
-                                                       i == 0 ? words(p.held) : nullptr);
+                                                       i == 0 ? words(p.held) : nullptr, words(p.joins),
+                                                       words(p.long_joins));
         in.keys = s.keys = keys;
         in.places = s.places = places;
         in.count = s.count;
@@ -708,11 +763,23 @@ b2_status b2_embedding(b2_ctx* ctx, const b2_embedding_args* args, const void* w
             const int ve = vector_width<T>(a.width, weight_stride, weight, rows);
             dispatch_vector<T>(ve, [&]<int VE>() {
                 const u32 columns = static_cast<u32>(a.width / VE);
-                const u64 blocks = ((a.count + kLookupRows - 1) / kLookupRows * columns + 255) / 256;
-                if (blocks >= 1ull << 31)
-                    throw Error(B2_CAPACITY, "b2_embedding: too many rows for one call");
-                k_lookup<T, VE><<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                    a, static_cast<const T*>(weight), weight_stride, static_cast<T*>(rows), columns);
+                auto launch = [&]<u32 ROWS>() {
+                    const u64 blocks = ((a.count + ROWS - 1) / ROWS * columns + 255) / 256;
+                    if (blocks >= 1ull << 31)
+                        throw Error(B2_CAPACITY, "b2_embedding: too many rows for one call");
+                    k_lookup<T, VE, ROWS><<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                        a, static_cast<const T*>(weight), weight_stride, static_cast<T*>(rows), columns);
+                };
+                // as many loads for a thread as leave the device its threads: eight rows from two full loads of it on
+                // (1.08 M rows of 128 fp32: 97 us, 105 with four), four for most (16,383 of 1,024 bf16: 12.5 us, 13.8
+                // with eight), one where a call's latency counts
+                const u64 vectors = a.count * columns, full = static_cast<u64>(ctx->sms) * 2048;
+                if (vectors >= 16 * full)
+                    launch.template operator()<8>();
+                else if (vectors >= full)
+                    launch.template operator()<4>();
+                else
+                    launch.template operator()<1>();
             });
             B2_CUDA(cudaGetLastError());
         });
@@ -763,10 +830,20 @@ b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, cons
             });
             if (s.chunks > 1)
             {
-                const dim3 grid(s.chunks, static_cast<unsigned>((a.width + kJoinColumns - 1) / kJoinColumns));
-                if (grid.y > 65535)
-                    throw Error(B2_CAPACITY, "b2_embedding_backward: rows of more than 8,388,480 columns");
-                k_segment_join<T><<<grid, 256, 0, st>>>(s, static_cast<T*>(grad_weight));
+                u32 slices = static_cast<u32>((a.width + kJoinColumns - 1) / kJoinColumns);
+                const u64 warps = static_cast<u64>(s.chunks) * slices;
+                T* const out = static_cast<T*>(grad_weight);
+                k_segment_join<T><<<grid_for(warps, 8, static_cast<unsigned>(ctx->sms) * 8), 256, 0, st>>>(s, out, slices);
+                if (s.chunks > kJoinShort + 1)
+                {
+                    u32 lanes = 1;
+                    while (lanes < 32 && lanes < a.width)
+                        lanes *= 2;
+                    slices = static_cast<u32>((a.width + lanes - 1) / lanes);
+                    const u64 blocks = static_cast<u64>(s.chunks) / (kJoinShort + 1) * slices;
+                    k_segment_join_long<T><<<grid_for(blocks, 1, static_cast<unsigned>(ctx->sms) * 4), 256, 0, st>>>(
+                        s, out, lanes, slices);
+                }
             }
             B2_CUDA(cudaGetLastError());
         });
