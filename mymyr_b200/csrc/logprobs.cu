@@ -61,7 +61,7 @@ struct Forward
     const void* tokens;
     int token_bits;
     u32 top;
-    float inv_t;
+    float inv_t, ahead;  // 1 / temperature; kAhead in units of the logits
     float *logprob, *entropy, *stats, *top_logprobs;
     long long* top_tokens;
 };
@@ -152,7 +152,7 @@ struct Row
     {
         log2_s = __log2f(a.s);
         log_s = dead ? -kInf : log2_s * kLn2;
-        entropy = dead ? 0.f : (log2_s - a.t / a.s) * kLn2;
+        entropy = dead ? 0.f : (log2_s - __fdividef(a.t, a.s)) * kLn2;
     }
     __device__ __forceinline__ float logp(float x) const
     {
@@ -214,15 +214,13 @@ __device__ __forceinline__ u64 warp_insert(u64 list, u64 key)
 
 // ---------------------------------------------------------------------------------------------- short rows
 
-/// `G` lanes for a row (one warp at most); up to R logits in each lane's registers, longer rows by reading them again.
+/// `G` lanes for a row; up to R logits in each lane's registers, longer rows by reading them again.
 template<class T, int G, int R>
 __global__ void __launch_bounds__(128) k_logprobs_short(const Forward a)
 {
     const u32 lane = threadIdx.x & (G - 1);
     const u64 r = (static_cast<u64>(blockIdx.x) * blockDim.x + threadIdx.x) / G;
     const bool live = r < a.count;
-    if (G == 32 && !live)
-        return;
     u64 begin = 0, mask_begin = 0;
     u32 len = 0;
     long long token = -1;
@@ -270,59 +268,32 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const Forward a)
         store_row(a, r, row, token, len, token >= 0 && token < len ? logit(static_cast<u32>(token)) : -kInf);
     if (!a.top)
         return;
-    if constexpr (G == 32)
+    u64 last = ~0ull;
+    for (u32 k = 0; k < a.top; ++k)
     {
-        u64 list = warp_sort(key_of(v[0], lane));
-        u64 least = __shfl_sync(~0u, list, a.top - 1);
-        auto offer = [&](u64 key) {
-            for (u32 more = __ballot_sync(~0u, key > least); more; more &= more - 1)
-            {
-                const u64 k = __shfl_sync(~0u, key, __ffs(more) - 1);
-                if (k > least)
-                {
-                    list = warp_insert(list, k);
-                    least = __shfl_sync(~0u, list, a.top - 1);
-                }
-            }
-        };
+        u64 best = 0;
 #pragma unroll
-        for (int i = 1; i < R; ++i)
-            if (i * G < len)
-                offer(key_of(v[i], i * G + lane));
-        for (u32 j = R * G; j < len; j += G)
-            offer(j + lane < len ? key_of(logit(j + lane), j + lane) : 0);
-        if (lane < a.top)
-            store_top(a, r, lane, row, list);
-    }
-    else
-    {
-        u64 last = ~0ull;
-        for (u32 k = 0; k < a.top; ++k)
+        for (int i = 0; i < R; ++i)
         {
-            u64 best = 0;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-            {
-                const u64 key = key_of(v[i], i * G + lane);
-                if (key < last && key > best)
-                    best = key;
-            }
-            for (u32 j = R * G + lane; j < len; j += G)
-            {
-                const u64 key = key_of(logit(j), j);
-                if (key < last && key > best)
-                    best = key;
-            }
-#pragma unroll
-            for (int o = G / 2; o; o /= 2)
-            {
-                const u64 other = __shfl_xor_sync(~0u, best, o);
-                best = other > best ? other : best;
-            }
-            last = best;
-            if (live && lane == 0)
-                store_top(a, r, k, row, best);
+            const u64 key = key_of(v[i], i * G + lane);
+            if (key < last && key > best)
+                best = key;
         }
+        for (u32 j = R * G + lane; j < len; j += G)
+        {
+            const u64 key = key_of(logit(j), j);
+            if (key < last && key > best)
+                best = key;
+        }
+#pragma unroll
+        for (int o = G / 2; o; o /= 2)
+        {
+            const u64 other = __shfl_xor_sync(~0u, best, o);
+            best = other > best ? other : best;
+        }
+        last = best;
+        if (live && lane == 0)
+            store_top(a, r, k, row, best);
     }
 }
 
@@ -540,22 +511,38 @@ __device__ __forceinline__ u64 block_merge(u64 list, u64* lists)
     return list;
 }
 
-/// A block (of NW warps) for a row, or the C blocks of a cluster for a row, each with a run of its vectors.
-template<class T, bool MASK, int NW>
-__global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 cluster)
+/// NW warps for a row, ROWS rows for a block (of one warp each where they are several); or a cluster of blocks for a row,
+/// each with a run of its vectors. A thread has U of them under way.
+template<class T, bool MASK, int NW, int U, int ROWS>
+__global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward a, u32 cluster)
 {
-    constexpr int VE = kVec<T>, N = NW * 32, U = 4;
-    constexpr u32 kFound = N;
-    __shared__ u64 lists[NW * kListKeys];
-    __shared__ u64 threshold_keys[kListKeys];
-    __shared__ u64 candidates[kFound];
-    __shared__ u32 held_keys, found;
-    __shared__ float4 sums[NW];  // of each warp
+    static_assert(NW == 1 || ROWS == 1);
+    constexpr int VE = kVec<T>, N = NW * 32;
+    constexpr u32 kFound = 256;
+    struct Shared
+    {
+        u64 lists[NW * kListKeys];
+        u64 threshold_keys[kListKeys];
+        u64 candidates[kFound];
+        float4 sums[NW];  // of each warp
+        u32 held_keys, found;
+    };
+    __shared__ Shared shared[ROWS];
     __shared__ float4 block_sums;
     __shared__ u64 block_list[kListKeys];
-    const u32 tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    const u64 r = blockIdx.x / cluster;
-    const u32 part = blockIdx.x % cluster;
+    const u32 lane = threadIdx.x & 31, w = NW == 1 ? 0 : threadIdx.x >> 5, tid = w * 32 + lane;
+    const u32 which = ROWS == 1 ? 0 : threadIdx.x >> 5;
+    auto& [lists, threshold_keys, candidates, sums, held_keys, found] = shared[which];
+    auto sync = [] {
+        if constexpr (NW == 1)
+            __syncwarp();
+        else
+            __syncthreads();
+    };
+    const u64 r = ROWS == 1 ? blockIdx.x / cluster : static_cast<u64>(blockIdx.x) * ROWS + which;
+    const u32 part = ROWS == 1 ? blockIdx.x % cluster : 0;
+    if (ROWS > 1 && r >= a.count)
+        return;
     u64 begin, mask_begin;
     u32 len;
     a.rows.at(r, begin, mask_begin, len);
@@ -573,7 +560,7 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
     const Vectors<T, MASK> row(x, mask, len);
     const u32 share = (row.count + cluster - 1) / cluster;
     const u32 first = min(part * share, row.count), last = min(first + share, row.count);
-    const float c = a.inv_t * kLog2e, ahead = kAhead / c;
+    const float c = a.inv_t * kLog2e, ahead = a.ahead;
     Scan<VE> scan;
     u32 i = first + tid;
     if (i < last && !row.whole(i))
@@ -602,13 +589,31 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
             scan.add(v, i + k * N, c, ahead);
         }
     }
-    for (; i < last; i += N)
+    if (i < whole_end)  // the last few, together as well
+    {
+        uint4 raw[U - 1];
+        u64 allowed[U - 1];
+#pragma unroll
+        for (int k = 0; k < U - 1; ++k)
+            if (i + k * N < whole_end)
+            {
+                raw[k] = row.load_raw(i + k * N);
+                allowed[k] = row.load_mask(i + k * N);
+            }
+#pragma unroll
+        for (int k = 0; k < U - 1; ++k)
+            if (i < whole_end)
+            {
+                float v[VE];
+                row.unpack(raw[k], allowed[k], v);
+                scan.add(v, i, c, ahead);
+                i += N;
+            }
+    }
+    if (i < last)
     {
         float v[VE];
-        if (i < whole_end)
-            row.unpack(row.load_raw(i), row.load_mask(i), v);
-        else
-            row.load_any(i, v);
+        row.load_any(i, v);
         scan.add(v, i, c, ahead);
     }
     // the block's sums about its largest logit
@@ -626,7 +631,7 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
         sum.t += __shfl_xor_sync(~0u, sum.t, o);
     }
     sum.best = best;
-    if (lane == 0)
+    if (NW > 1 && lane == 0)
         sums[w] = sum.pack();
     u64 list = 0;
     if (a.top)
@@ -644,7 +649,7 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
             }
         }
     }
-    __syncthreads();
+    sync();
     if (a.top)
     {
         // the logits of the best threads (every N-th vector), those that reach the bound; as many as a thread can hold
@@ -670,13 +675,18 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
                     candidates[to] = key;
             }
         }
-        __syncthreads();
-        if (found <= kFound)
+        sync();
+        const u32 got = found;
+        if (got <= kFound)
         {
-            // sorted by as many warps as they fill
-            const u32 at = w * 32 + lane;
-            list = w * 32 < found || w == 0 ? warp_sort(at < found ? candidates[at] : 0) : 0;
-            if (found > 32)
+            // sorted 32 by each warp
+            list = 0;
+            for (u32 at = w * 32; at < got; at += N)
+            {
+                const u64 more = warp_sort(at + lane < got ? candidates[at + lane] : 0);
+                list = at < static_cast<u32>(N) ? more : warp_merge(list, __shfl_sync(~0u, more, 31 - lane));
+            }
+            if (NW > 1 && got > 32)
                 list = block_merge<NW>(list, lists);
         }
         else
@@ -713,13 +723,13 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
             list = block_merge<NW>(list, lists);
         }
     }
-    if (w == 0)
+    if (NW > 1 && w == 0)
     {
         sum = Sums(sums[0]);
         for (int k = 1; k < NW; ++k)
             sum.join(Sums(sums[k]), c);
     }
-    if (cluster > 1)
+    if (ROWS == 1 && NW > 1 && cluster > 1)
     {
         cg::cluster_group group = cg::this_cluster();
         if (w == 0)
@@ -751,48 +761,63 @@ __global__ void __launch_bounds__(NW * 32) k_logprobs_long(const Forward a, u32 
 
 constexpr int kBackwardBlock = 256, kBackwardVectors = 4;
 
-template<class T, bool MASK>
-__global__ void __launch_bounds__(kBackwardBlock, MASK ? 4 : 8) k_logprobs_backward_long(const Backward a)
+/// A row's logits and the gradient's, for N threads that take its vectors.
+template<class T, bool MASK, int N>
+struct Gradient
 {
-    constexpr int VE = kVec<T>, U = kBackwardVectors;
+    static constexpr int VE = kVec<T>, U = kBackwardVectors;
     struct alignas(16) Out
     {
         T v[VE];
     };
-    zero_outside<T>(a);
-    const u64 r = blockIdx.x / a.slices;
-    u64 begin, mask_begin;
-    u32 len;
-    a.rows.at(r, begin, mask_begin, len);
-    const Vectors<T, MASK> row(static_cast<const T*>(a.rows.logits) + begin,
-                               MASK ? a.rows.mask + mask_begin : nullptr, len);
-    T* const dx = static_cast<T*>(a.grad) + (a.rows.offsets ? begin : r * a.grad_stride) - row.shift;
-    const bool aligned = reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+    Vectors<T, MASK> row;
     long long token;
-    const Slope slope(a, r, token, len);
-    const u32 own_at = token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u;
-    const u32 whole_begin = row.shift ? 1 : 0, whole_end = row.end / VE;
-    auto slopes = [&](float(&v)[VE]) {
+    Slope slope;
+    T* dx;  // of vector 0's first element
+    bool aligned;
+    u32 own_at, whole_begin, whole_end;
+
+    __device__ __forceinline__ Gradient(const Backward& a, u64 r, u64 begin, u64 mask_begin, u32 len)
+        : row(static_cast<const T*>(a.rows.logits) + begin, MASK ? a.rows.mask + mask_begin : nullptr, len),
+          slope(a, r, token, len),
+          dx(static_cast<T*>(a.grad) + (a.rows.offsets ? begin : r * a.grad_stride) - row.shift),
+          aligned(reinterpret_cast<uintptr_t>(dx) % 16 == 0),
+          own_at(token >= 0 && token < len ? static_cast<u32>(token) + row.shift : ~0u),
+          whole_begin(row.shift ? 1 : 0),
+          whole_end(row.end / VE)
+    {
+    }
+    __device__ __forceinline__ void slopes(float (&v)[VE]) const
+    {
 #pragma unroll
         for (int q = 0; q < VE; ++q)
         {
             const float g = slope(v[q]);
             v[q] = MASK && v[q] == -kInf ? 0.f : g;
         }
-    };
-    for (u64 i0 = (blockIdx.x % a.slices) * static_cast<u64>(kBackwardBlock * U); i0 < row.count;
-         i0 += static_cast<u64>(a.slices) * kBackwardBlock * U)
+    }
+    __device__ __forceinline__ void store(const float (&v)[VE], u32 j) const
     {
-        const u32 i = static_cast<u32>(i0) + threadIdx.x;
-        if (aligned && !slope.dead && i0 >= whole_begin && i0 + kBackwardBlock * U <= whole_end)
+        Out o;
+#pragma unroll
+        for (int q = 0; q < VE; ++q)
+            o.v[q] = from_f32<T>(v[q]);
+        *reinterpret_cast<Out*>(dx + static_cast<u64>(j) * VE) = o;
+    }
+    /// The N * U vectors from i0 on.
+    __device__ __forceinline__ void write(u64 i0, u32 thread) const
+    {
+        const u32 i = static_cast<u32>(i0) + thread;
+        const bool plain = aligned && !slope.dead;
+        if (plain && i0 >= whole_begin && i0 + N * U <= whole_end)
         {
             uint4 raw[U];
             u64 allowed[U];
 #pragma unroll
             for (int k = 0; k < U; ++k)
             {
-                raw[k] = row.load_raw(i + k * kBackwardBlock);
-                allowed[k] = row.load_mask(i + k * kBackwardBlock);
+                raw[k] = row.load_raw(i + k * N);
+                allowed[k] = row.load_mask(i + k * N);
             }
 #pragma unroll
             for (int k = 0; k < U; ++k)
@@ -800,30 +825,89 @@ __global__ void __launch_bounds__(kBackwardBlock, MASK ? 4 : 8) k_logprobs_backw
                 float v[VE];
                 row.unpack(raw[k], allowed[k], v);
                 slopes(v);
-                Out o;
-#pragma unroll
-                for (int q = 0; q < VE; ++q)
-                    o.v[q] = from_f32<T>(v[q]);
-                *reinterpret_cast<Out*>(dx + static_cast<u64>(i + k * kBackwardBlock) * VE) = o;
+                store(v, i + k * N);
             }
         }
         else
-            for (u32 j = i; j < min(i0 + kBackwardBlock * U, static_cast<u64>(row.count)); j += kBackwardBlock)
+        {
+            // a row's ends, rows that leave nothing, a gradient of another alignment; whole vectors still G at a time (a
+            // warp comes here with most of a short row; the larger blocks would lack the registers for more)
+            constexpr int G = N == 32 ? U : 1;
+#pragma unroll 1
+            for (int first = 0; first < U; first += G)
             {
-                float v[VE];
-                row.load_any(j, v);
-                slopes(v);
+                uint4 raw[G];
+                u64 allowed[G];
 #pragma unroll
-                for (int q = 0; q < VE; ++q)
-                    if (j * VE + q >= row.shift && j * VE + q < row.end)
-                        dx[static_cast<u64>(j) * VE + q] = from_f32<T>(slope.dead ? 0.f : v[q]);
+                for (int k = 0; k < G; ++k)
+                {
+                    const u32 j = i + (first + k) * N;
+                    if (plain && j >= whole_begin && j < whole_end)
+                    {
+                        raw[k] = row.load_raw(j);
+                        allowed[k] = row.load_mask(j);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < G; ++k)
+                {
+                    const u32 j = i + (first + k) * N;
+                    float v[VE];
+                    if (plain && j >= whole_begin && j < whole_end)
+                    {
+                        row.unpack(raw[k], allowed[k], v);
+                        slopes(v);
+                        store(v, j);
+                    }
+                    else if (j < row.count)
+                    {
+                        row.load_any(j, v);
+                        slopes(v);
+#pragma unroll
+                        for (int q = 0; q < VE; ++q)
+                            if (j * VE + q >= row.shift && j * VE + q < row.end)
+                                dx[static_cast<u64>(j) * VE + q] = from_f32<T>(slope.dead ? 0.f : v[q]);
+                    }
+                }
             }
+        }
         // the given token's own part, by the thread that has just written its vector
         const u32 at = own_at / VE - static_cast<u32>(i0);
-        if (own_at != ~0u && at < kBackwardBlock * U && at % kBackwardBlock == threadIdx.x && !slope.dead &&
-            (!MASK || row.mask[own_at]))
+        if (own_at != ~0u && at < N * U && at % N == thread && !slope.dead && (!MASK || row.mask[own_at]))
             dx[own_at] = from_f32<T>(slope(to_f32(row.base[own_at])) + slope.own);
     }
+};
+
+/// A warp for a row.
+template<class T, bool MASK>
+__global__ void __launch_bounds__(kBackwardBlock, 4) k_logprobs_backward_warp(const Backward a)
+{
+    zero_outside<T>(a);
+    const u64 r = (static_cast<u64>(blockIdx.x) * kBackwardBlock + threadIdx.x) / 32;
+    if (r >= a.count)
+        return;
+    u64 begin, mask_begin;
+    u32 len;
+    a.rows.at(r, begin, mask_begin, len);
+    const Gradient<T, MASK, 32> gradient(a, r, begin, mask_begin, len);
+    for (u64 i0 = 0; i0 < gradient.row.count; i0 += 32 * kBackwardVectors)
+        gradient.write(i0, threadIdx.x & 31);
+}
+
+/// `slices` blocks for a row. Each SM is full of them: 8192 rows of 65,536 bf16 take 317 us (6.8 TB/s), with six blocks
+/// an SM 350.
+template<class T, bool MASK>
+__global__ void __launch_bounds__(kBackwardBlock, MASK ? 4 : 8) k_logprobs_backward_long(const Backward a)
+{
+    zero_outside<T>(a);
+    const u64 r = blockIdx.x / a.slices;
+    u64 begin, mask_begin;
+    u32 len;
+    a.rows.at(r, begin, mask_begin, len);
+    const Gradient<T, MASK, kBackwardBlock> gradient(a, r, begin, mask_begin, len);
+    constexpr u64 kSlice = static_cast<u64>(kBackwardBlock) * kBackwardVectors;
+    for (u64 i0 = (blockIdx.x % a.slices) * kSlice; i0 < gradient.row.count; i0 += a.slices * kSlice)
+        gradient.write(i0, threadIdx.x);
 }
 
 Rows rows_of(const b2_logprobs_args& a)
@@ -834,14 +918,35 @@ Rows rows_of(const b2_logprobs_args& a)
 /// The mean length of a call's rows, by which they are laid out (ragged rows that are longer still are right, if slower).
 u64 mean_length(const Rows& rows, u64 count) { return rows.offsets ? rows.width / count : rows.width; }
 
-constexpr u64 kShort = 1024;
+/// How a call's rows are laid out.
+enum class Layout
+{
+    lanes4,  // a group of lanes for a row, up to 8 or 16 logits for a lane
+    lanes8,
+    warp,    // a warp for a row, in vectors of 16 bytes
+    block    // a block or more
+};
 
-template<class T, bool MASK, int NW>
+/// By the mean length. Few lanes with many logits each cost less than many with few: most of a short row's instructions
+/// are its sums over the lanes and its results (65,536 rows of 100 bf16: 16 us forward, with 32 lanes 41). A warp takes
+/// vectors, 32 at a time, while a row has few or the rows fill the device with warps.
+template<class T>
+Layout layout_of(const b2_ctx& ctx, const Rows& rows, u64 count)
+{
+    const u64 mean = mean_length(rows, count), vectors = mean / kVec<T>;
+    if (mean <= 32)
+        return Layout::lanes4;
+    if (mean <= 128)
+        return Layout::lanes8;
+    return vectors <= 256 || (vectors <= 1024 && count >= static_cast<u64>(ctx.sms) * 16) ? Layout::warp : Layout::block;
+}
+
+template<class T, bool MASK, int NW, int U, int ROWS>
 void forward_long(const Forward& f, u32 cluster, cudaStream_t st)
 {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(f.count) * cluster);
-    cfg.blockDim = dim3(NW * 32);
+    cfg.gridDim = dim3(static_cast<unsigned>((f.count + ROWS - 1) / ROWS) * cluster);
+    cfg.blockDim = dim3(NW * ROWS * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -849,23 +954,22 @@ void forward_long(const Forward& f, u32 cluster, cudaStream_t st)
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    B2_CUDA(cudaLaunchKernelEx(&cfg, k_logprobs_long<T, MASK, NW>, f, cluster));
+    B2_CUDA(cudaLaunchKernelEx(&cfg, k_logprobs_long<T, MASK, NW, U, ROWS>, f, cluster));
 }
 
 template<class T>
 void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
 {
     const u64 mean = mean_length(f.rows, f.count);
-    if (mean <= kShort)
+    auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
+    switch (layout_of<T>(ctx, f.rows, f.count))
     {
-        auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
-        if (mean <= 4)
-            k_logprobs_short<T, 4, 4><<<blocks(4), 128, 0, st>>>(f);
-        else if (mean <= 16)
-            k_logprobs_short<T, 8, 8><<<blocks(8), 128, 0, st>>>(f);
-        else
-            k_logprobs_short<T, 32, 32><<<blocks(32), 128, 0, st>>>(f);
-        return;
+        case Layout::lanes4: k_logprobs_short<T, 4, 8><<<blocks(4), 128, 0, st>>>(f); return;
+        case Layout::lanes8: k_logprobs_short<T, 8, 16><<<blocks(8), 128, 0, st>>>(f); return;
+        case Layout::warp:
+            f.rows.mask ? forward_long<T, true, 1, 4, 8>(f, 1, st) : forward_long<T, false, 1, 4, 8>(f, 1, st);
+            return;
+        case Layout::block: break;
     }
     // blocks of 8 warps; a cluster for a row while its blocks still have two vectors for each thread and the device
     // has room for all of them at twice a block for each SM
@@ -874,35 +978,48 @@ void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
     while (cluster < 8 && f.count * cluster * 2 <= static_cast<u64>(ctx.sms) * 2 &&
            mean >= static_cast<u64>(cluster) * 2 * NW * 32 * kVec<T> * 2)
         cluster *= 2;
-    if (f.rows.mask)
-        forward_long<T, true, NW>(f, cluster, st);
-    else
-        forward_long<T, false, NW>(f, cluster, st);
+    // a cluster's threads have few vectors each: all of them at once; blocks of 4 warps where rows are many and not long
+    // enough to make up for what a larger block waits for at their ends (16,384 rows of 15,000 bf16: 102 us, with 8 warps
+    // 134; 2,048 of 50,001 fp32 with 8 alternatives: 106 and 84), nor many alternatives to be looked for among few
+    // threads' logits (16,384 of 30,001 bf16 with 20: 344 and 314)
+    const bool few_warps = f.count >= static_cast<u64>(ctx.sms) * 8 && f.top <= 8 &&
+                           mean <= (f.top ? 4096u : 8192u) * kVec<T>;
+    auto run = [&]<bool MASK>() {
+        if (cluster > 1)
+            forward_long<T, MASK, NW, 8, 1>(f, cluster, st);
+        else if (few_warps)
+            forward_long<T, MASK, 4, 4, 1>(f, 1, st);
+        else
+            forward_long<T, MASK, NW, 4, 1>(f, 1, st);
+    };
+    f.rows.mask ? run.template operator()<true>() : run.template operator()<false>();
 }
 
 template<class T>
-void backward(Backward f, cudaStream_t st)
+void backward(const b2_ctx& ctx, Backward f, cudaStream_t st)
 {
     const u64 mean = mean_length(f.rows, f.count);
-    if (mean <= kShort)
+    auto blocks = [&](u64 lanes, u64 threads) { return static_cast<unsigned>((f.count * lanes + threads - 1) / threads); };
+    switch (layout_of<T>(ctx, f.rows, f.count))
     {
-        auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
-        if (mean <= 4)
-            k_logprobs_backward_short<T, 4><<<blocks(4), 128, 0, st>>>(f);
-        else if (mean <= 16)
-            k_logprobs_backward_short<T, 8><<<blocks(8), 128, 0, st>>>(f);
-        else
-            k_logprobs_backward_short<T, 32><<<blocks(32), 128, 0, st>>>(f);
-        return;
+        case Layout::lanes4: k_logprobs_backward_short<T, 4><<<blocks(4, 128), 128, 0, st>>>(f); return;
+        case Layout::lanes8: k_logprobs_backward_short<T, 8><<<blocks(8, 128), 128, 0, st>>>(f); return;
+        case Layout::warp:
+            if (f.rows.mask)
+                k_logprobs_backward_warp<T, true><<<blocks(32, kBackwardBlock), kBackwardBlock, 0, st>>>(f);
+            else
+                k_logprobs_backward_warp<T, false><<<blocks(32, kBackwardBlock), kBackwardBlock, 0, st>>>(f);
+            return;
+        case Layout::block: break;
     }
     constexpr u64 slice = static_cast<u64>(kBackwardBlock) * kBackwardVectors * kVec<T>;
     const u64 most = ((1ull << 31) - 1) / f.count;
     f.slices = static_cast<u32>(std::max<u64>(1, std::min<u64>((mean + slice - 1) / slice, most)));
-    const unsigned blocks = static_cast<unsigned>(f.count * f.slices);
+    const unsigned grid = static_cast<unsigned>(f.count * f.slices);
     if (f.rows.mask)
-        k_logprobs_backward_long<T, true><<<blocks, kBackwardBlock, 0, st>>>(f);
+        k_logprobs_backward_long<T, true><<<grid, kBackwardBlock, 0, st>>>(f);
     else
-        k_logprobs_backward_long<T, false><<<blocks, kBackwardBlock, 0, st>>>(f);
+        k_logprobs_backward_long<T, false><<<grid, kBackwardBlock, 0, st>>>(f);
 }
 
 void check_args(b2_ctx* ctx, const b2_logprobs_args* a, const char* what)
@@ -941,7 +1058,8 @@ b2_status b2_logprobs(b2_ctx* ctx, const b2_logprobs_args* args, void* stream)
             if (!a.rows)
                 return;
             const OnDevice on(ctx->device);
-            const Forward f{rows_of(a), a.rows, a.tokens, a.token_bits, a.top, 1.f / a.temperature, a.logprob, a.entropy, a.stats,
+            const Forward f{rows_of(a), a.rows, a.tokens, a.token_bits, a.top, 1.f / a.temperature,
+                            kAhead / (1.f / a.temperature * kLog2e), a.logprob, a.entropy, a.stats,
                             a.top_logprobs, reinterpret_cast<long long*>(a.top_tokens)};
             forward<T>(*ctx, f, static_cast<cudaStream_t>(stream));
             B2_CUDA(cudaGetLastError());
@@ -963,7 +1081,7 @@ b2_status b2_logprobs_backward(b2_ctx* ctx, const b2_logprobs_args* args, const 
             const OnDevice on(ctx->device);
             const Backward f{rows_of(a), a.rows, a.tokens, a.token_bits, 1, 1.f / a.temperature, a.stats,
                              a.tokens ? grad_logprob : nullptr, grad_entropy, grad_logits, grad_stride};
-            backward<T>(f, static_cast<cudaStream_t>(stream));
+            backward<T>(*ctx, f, static_cast<cudaStream_t>(stream));
             B2_CUDA(cudaGetLastError());
         });
     });
