@@ -16,6 +16,7 @@ constexpr u32 kWarps = 8;
 struct Hyper
 {
     float b1, a1, b2, a2, decay, correct, eps, rate;
+    float one;  // 1: a sum of two products written as a fused multiplication by it is not fused with either of them
 };
 
 struct Moments
@@ -117,13 +118,17 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8])
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-/// Fast square root and reciprocal of normal numbers (2 units in the last place).
-__device__ __forceinline__ float sqrt_fast(float x)
+/// The square root of a normal number to 2 units in the last place, and what a step of Heron's rule adds to it: their sum
+/// is rounded correctly but for a few in a thousand.
+__device__ __forceinline__ float sqrt_fast(float x, float& rest)
 {
-    float r;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    const float r = x * y;
+    rest = fmaf(-r, r, x) * (0.5f * y);
     return r;
 }
+/// The reciprocal of a normal number to 2 units in the last place.
 __device__ __forceinline__ float reciprocal_fast(float x)
 {
     float r;
@@ -205,11 +210,10 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
             (t.e[mid].begin <= b ? entry : hi) = mid;
         }
     }
-    const Two b1(h.b1, h.b1), a1(h.a1, h.a1), b2(h.b2, h.b2), a2(h.a2, h.a2);
+    const Two b1(h.b1, h.b1), a1(h.a1, h.a1), b2(h.b2, h.b2), a2(h.a2, h.a2), one(h.one, h.one);
     P* p = nullptr;
     const G* g = nullptr;
-    M *m_at = nullptr, *v_at = nullptr;
-    float* master = nullptr;
+    u64 at = 0;    // in the moments, which hold whole blocks
     u64 left = 0;  // elements of the tensor from this block on
     u32 block = 0, next_entry = b;
     bool aligned = false;
@@ -223,15 +227,15 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
             next_entry = entry + 1 < t.count ? t.e[entry + 1].begin : ~0u;
             block = e.block + (b - e.begin);
             const u64 first = static_cast<u64>(b - e.begin) * kMoment;  // in the tensor
-            const u64 at = static_cast<u64>(block) * kMoment + i0;      // in the moments, which hold whole blocks
+            at = static_cast<u64>(block) * kMoment + i0;
             left = e.n - first;
             p = static_cast<P*>(e.p) + first + i0;
             g = static_cast<const G*>(e.g) + first + i0;
-            m_at = static_cast<M*>(s.m) + at;
-            v_at = static_cast<M*>(s.v) + at;
-            master = s.master + at;
             aligned = !(reinterpret_cast<uintptr_t>(e.p) & kAlign8<P>) && !(reinterpret_cast<uintptr_t>(e.g) & kAlign8<G>);
         }
+        M* const m_at = static_cast<M*>(s.m) + at;
+        M* const v_at = static_cast<M*>(s.v) + at;
+        float* const master = s.master + at;
         // a tensor's last block, and tensors that start off a vector's boundary, go element by element
         const u32 n = static_cast<u32>(min(left, static_cast<u64>(kMoment)));
         const bool whole = aligned && n == kMoment;
@@ -278,8 +282,8 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
         for (int k = 0; k < 8; k += 2)
         {
             const Two g2(gi[k], gi[k + 1]);
-            const float2 x = (Two(m[k], m[k + 1]) * b1 + g2 * a1).get();
-            const float2 y = (Two(v[k], v[k + 1]) * b2 + g2 * g2 * a2).get();
+            const float2 x = fma(Two(m[k], m[k + 1]) * b1, one, g2 * a1).get();
+            const float2 y = fma(Two(v[k], v[k + 1]) * b2, one, g2 * g2 * a2).get();
             m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
         }
         float m_most = 0.f, v_most = 0.f;
@@ -289,8 +293,11 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
             // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
             float floor;
             asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
-            r[k] = sqrt_fast(floor);
-            now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(r[k] * h.correct + h.eps));
+            float rest;
+            const float root = sqrt_fast(floor, rest);
+            // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
+            r[k] = BITS == 8 ? root + rest : root;
+            now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
             if constexpr (BITS == 8)
             {
                 m_most = max_magnitude(m_most, m[k]);
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
                 s.v_scale[block] = vs;
             }
         }
-        p += kMoment, g += kMoment, m_at += kMoment, v_at += kMoment, master += kMoment;
+        p += kMoment, g += kMoment, at += kMoment;
         left -= n, ++block;
     }
 }
@@ -385,8 +392,8 @@ void launch(const b2_ctx& ctx, const b2_adamw_args& a, u32 first, u32 count, con
     t.blocks = static_cast<u32>(blocks);
     const u32 key = mix(mix(a.seed) ^ static_cast<u32>(a.step));
     const Moments s{a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.master};
-    // runs of up to eight blocks, while the warps that the device holds have four each
-    const u32 run = static_cast<u32>(std::min<u64>(8, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 128))));
+    // runs of up to 32 blocks, while the warps that the device holds have four each
+    const u32 run = static_cast<u32>(std::min<u64>(32, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 128))));
     const u64 per = static_cast<u64>(kWarps) * run;
     k_adamw<P, G, BITS, MASTER, N>
         <<<static_cast<unsigned>((blocks + per - 1) / per), kWarps * 32, 0, st>>>(t, s, h, key, run);
@@ -400,7 +407,7 @@ void run(const b2_ctx& ctx, const b2_adamw_args& a, cudaStream_t st)
     const double c2 = 1 - std::pow(a.beta2, static_cast<double>(a.step));
     const Hyper h{static_cast<float>(a.beta1), static_cast<float>(1 - a.beta1), static_cast<float>(a.beta2),
                   static_cast<float>(1 - a.beta2), static_cast<float>(1 - a.lr * a.weight_decay),
-                  static_cast<float>(1 / std::sqrt(c2)), static_cast<float>(a.eps), static_cast<float>(a.lr / c1)};
+                  static_cast<float>(1 / std::sqrt(c2)), static_cast<float>(a.eps), static_cast<float>(a.lr / c1), 1.f};
     constexpr u32 kFew = 96, kMany = 1000;
     for (u32 first = 0; first < a.count;)
     {
