@@ -513,7 +513,7 @@ __device__ __forceinline__ u64 block_merge(u64 list, u64* lists)
 
 /// NW warps for a row, ROWS rows for a block (of one warp each where they are several); or a cluster of blocks for a row,
 /// each with a run of its vectors. A thread has U of them under way.
-template<class T, bool MASK, int NW, int U, int ROWS>
+template<class T, bool MASK, bool TOP, int NW, int U, int ROWS>
 __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward a, u32 cluster)
 {
     static_assert(NW == 1 || ROWS == 1);
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward 
     if (NW > 1 && lane == 0)
         sums[w] = sum.pack();
     u64 list = 0;
-    if (a.top)
+    if constexpr (TOP)
     {
         // the threads' best; the top-th of them bounds what can be among the row's best
         list = block_merge<NW>(warp_sort(key_of(scan.best, scan.at)), lists);
@@ -650,34 +650,71 @@ __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward 
         }
     }
     sync();
-    if (a.top)
+    if constexpr (TOP)
     {
-        // the logits of the best threads (every N-th vector), those that reach the bound; as many as a thread can hold
-        // each are seldom more than the alternatives themselves
+        // The logits of the best threads (every N-th vector), those that reach the bound: seldom many more than the
+        // alternatives themselves. Two of a thread's vectors are under way at a time.
         const u64 bound = threshold_keys[a.top - 1];
+        const float least = logit_of(bound);
         const u32 each = (last - first + N - 1) / N, pairs = min(a.top, held_keys) * each;
-        for (u32 p = tid; p < pairs; p += N)
+        auto vector_of = [&](u32 p) {
+            return p < pairs ? first + (index_of(threshold_keys[p / each]) - first) % N + p % each * N : last;
+        };
+        if (tid < kListKeys)
+            lists[tid] = 0;
+        for (u32 p = tid; p < pairs; p += 2 * N)
         {
-            const u32 j = first + (index_of(threshold_keys[p / each]) - first) % N + p % each * N;
-            if (j >= last)
-                continue;
-            float v[VE];
-            row.load_any(j, v);
-            if (key_of(max_of(v), j) < bound)
-                continue;
-            for (int q = 0; q < VE; ++q)
+            float v[2][VE];
+            const u32 j[2] = {vector_of(p), vector_of(p + N)};
+            uint4 raw[2];
+            u64 allowed[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (j[k] < last && row.whole(j[k]))
+                {
+                    raw[k] = row.load_raw(j[k]);
+                    allowed[k] = row.load_mask(j[k]);
+                }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
             {
-                const u64 key = key_of(v[q], j * VE - row.shift + q);
-                if (!key || (key | ~0u) < bound)  // a smaller logit than the bound's
+                if (j[k] >= last)
                     continue;
-                const u32 to = atomicAdd(&found, 1u);
-                if (to < kFound)
-                    candidates[to] = key;
+                if (row.whole(j[k]))
+                    row.unpack(raw[k], allowed[k], v[k]);
+                else
+                    row.load_any(j[k], v[k]);
+                if (max_of(v[k]) < least)
+                    continue;
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    if (v[k][q] >= least && v[k][q] > -kInf)
+                    {
+                        const u32 to = atomicAdd(&found, 1u);
+                        if (to < kFound)
+                            candidates[to] = key_of(v[k][q], j[k] * VE - row.shift + q);
+                    }
             }
         }
         sync();
         const u32 got = found;
-        if (got <= kFound)
+        if ((got + N - 1) / N * got <= (NW == 1 ? 128 : 256))
+        {
+            // each of them counts the larger ones: its place
+            for (u32 at = tid; at < got; at += N)
+            {
+                const u64 key = candidates[at];
+                u32 larger = 0;
+#pragma unroll 4
+                for (u32 k = 0; k < got; ++k)
+                    larger += candidates[k] > key;
+                if (larger < kListKeys)
+                    lists[larger] = key;
+            }
+            sync();
+            list = lists[lane];
+        }
+        else if (got <= kFound)
         {
             // sorted 32 by each warp
             list = 0;
@@ -686,7 +723,7 @@ __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward 
                 const u64 more = warp_sort(at + lane < got ? candidates[at + lane] : 0);
                 list = at < static_cast<u32>(N) ? more : warp_merge(list, __shfl_sync(~0u, more, 31 - lane));
             }
-            if (NW > 1 && got > 32)
+            if (NW > 1)
                 list = block_merge<NW>(list, lists);
         }
         else
@@ -744,7 +781,7 @@ __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward 
             if (w == 0)
                 for (u32 k = 1; k < cluster; ++k)
                     sum.join(Sums(*group.map_shared_rank(&block_sums, k)), c);
-            if (a.top)  // a warp for each block's list
+            if constexpr (TOP)  // a warp for each block's list
                 list = block_merge<NW>(w < cluster ? group.map_shared_rank(block_list, w)[lane] : 0, lists);
         }
         group.sync();  // the other blocks' shared memory stays until it has been read
@@ -754,7 +791,7 @@ __global__ void __launch_bounds__(NW * ROWS * 32) k_logprobs_long(const Forward 
         const Row out(sum, a.inv_t);
         if (lane == 0)
             store_row(a, r, out, token, len, given);
-        if (lane < a.top)
+        if (TOP && lane < a.top)
             store_top(a, r, lane, out, list);
     }
 }
@@ -941,7 +978,7 @@ Layout layout_of(const b2_ctx& ctx, const Rows& rows, u64 count)
     return vectors <= 256 || (vectors <= 1024 && count >= static_cast<u64>(ctx.sms) * 16) ? Layout::warp : Layout::block;
 }
 
-template<class T, bool MASK, int NW, int U, int ROWS>
+template<class T, bool MASK, bool TOP, int NW, int U, int ROWS>
 void forward_long(const Forward& f, u32 cluster, cudaStream_t st)
 {
     cudaLaunchConfig_t cfg{};
@@ -954,7 +991,7 @@ void forward_long(const Forward& f, u32 cluster, cudaStream_t st)
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    B2_CUDA(cudaLaunchKernelEx(&cfg, k_logprobs_long<T, MASK, NW, U, ROWS>, f, cluster));
+    B2_CUDA(cudaLaunchKernelEx(&cfg, k_logprobs_long<T, MASK, TOP, NW, U, ROWS>, f, cluster));
 }
 
 template<class T>
@@ -962,12 +999,18 @@ void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
 {
     const u64 mean = mean_length(f.rows, f.count);
     auto blocks = [&](u64 lanes) { return static_cast<unsigned>((f.count * lanes + 127) / 128); };
+    auto with_flags = [&](auto&& run) {
+        if (f.rows.mask)
+            f.top ? run.template operator()<true, true>() : run.template operator()<true, false>();
+        else
+            f.top ? run.template operator()<false, true>() : run.template operator()<false, false>();
+    };
     switch (layout_of<T>(ctx, f.rows, f.count))
     {
         case Layout::lanes4: k_logprobs_short<T, 4, 8><<<blocks(4), 128, 0, st>>>(f); return;
         case Layout::lanes8: k_logprobs_short<T, 8, 16><<<blocks(8), 128, 0, st>>>(f); return;
         case Layout::warp:
-            f.rows.mask ? forward_long<T, true, 1, 4, 8>(f, 1, st) : forward_long<T, false, 1, 4, 8>(f, 1, st);
+            with_flags([&]<bool MASK, bool TOP>() { forward_long<T, MASK, TOP, 1, 4, 8>(f, 1, st); });
             return;
         case Layout::block: break;
     }
@@ -984,15 +1027,14 @@ void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
     // threads' logits (16,384 of 30,001 bf16 with 20: 344 and 314)
     const bool few_warps = f.count >= static_cast<u64>(ctx.sms) * 8 && f.top <= 8 &&
                            mean <= (f.top ? 4096u : 8192u) * kVec<T>;
-    auto run = [&]<bool MASK>() {
+    with_flags([&]<bool MASK, bool TOP>() {
         if (cluster > 1)
-            forward_long<T, MASK, NW, 8, 1>(f, cluster, st);
+            forward_long<T, MASK, TOP, NW, 8, 1>(f, cluster, st);
         else if (few_warps)
-            forward_long<T, MASK, 4, 4, 1>(f, 1, st);
+            forward_long<T, MASK, TOP, 4, 4, 1>(f, 1, st);
         else
-            forward_long<T, MASK, NW, 4, 1>(f, 1, st);
-    };
-    f.rows.mask ? run.template operator()<true>() : run.template operator()<false>();
+            forward_long<T, MASK, TOP, NW, 4, 1>(f, 1, st);
+    });
 }
 
 template<class T>
