@@ -514,8 +514,11 @@ typedef struct b2_adamw_args {
 } b2_adamw_args;
 
 /* m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2; p = p (1 - lr weight_decay) - lr m' / (sqrt(v') + eps)
- * with m' = m / (1 - beta1^step), v' = v / (1 - beta2^step), in 32 bits, for every tensor: one launch for up to 96
- * tensors or each 1,000 of them. */
+ * with m' = m / (1 - beta1^step), v' = v / (1 - beta2^step), in 32 bits, for every tensor: one launch for each 1,000 of
+ * them. 8-bit moments are rounded when they are stored: the first to the nearest code, the second (its square root) to
+ * one of the two codes about it, at random by (seed, step, element) with the odds that keep the mean of its square; a
+ * positive one of at least 2^-126 keeps at least the smallest code. A parameter with a NaN or infinite gradient becomes
+ * NaN or infinite and leaves the others of its block alone. */
 b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -512,11 +512,12 @@ __device__ __forceinline__ u64 block_merge(u64 list, u64* lists)
 }
 
 /// NW warps for a row, ROWS rows for a block (of one warp each where they are several); or a cluster of blocks for a row,
-/// each with a run of its vectors. A thread has U of them under way; forty warps an SM, but where U is 8 (a cluster's few
-/// rows wait for latency alone). 8,192 rows of 65,536 bf16: 186 us (5.8 TB/s); 2,048 of 50,001 fp32 with 8 alternatives:
-/// 77 us (5.3 TB/s), of which the alternatives 7; one row of 131,072 bf16 with 20: 7.8 us, of which the alternatives 3.
+/// each with a run of its vectors. A thread has U of them under way; forty warps an SM, fewer where U is 8 (a cluster's
+/// few rows wait for latency, not for bandwidth). 8,192 rows of 65,536 bf16: 186 us (5.8 TB/s); 2,048 of 50,001 fp32 with
+/// 8 alternatives: 77 us (5.3 TB/s), of which the alternatives 7; one row of 131,072 bf16 with 20: 7.6 us, of which the
+/// alternatives 3.
 template<class T, bool MASK, bool TOP, int NW, int U, int ROWS>
-__global__ void __launch_bounds__(NW * ROWS * 32, U == 8 ? 1 : 40 / (NW * ROWS)) k_logprobs_long(const Forward a, u32 cluster)
+__global__ void __launch_bounds__(NW * ROWS * 32, U == 8 ? 3 : 40 / (NW * ROWS)) k_logprobs_long(const Forward a, u32 cluster)
 {
     static_assert(NW == 1 || ROWS == 1);
     constexpr int VE = kVec<T>, N = NW * 32;

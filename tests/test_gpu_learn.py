@@ -778,3 +778,29 @@ def test_actions_of_an_expansion():
     near(got.logprob, -count.log(), 8 * EPS)
     near(got.entropy, count.log(), 8 * EPS)
     assert torch.equal((got.top_tokens >= 0).sum(1), count.long())
+
+
+def test_gradients_of_gradients_are_refused():
+    x, w = randn(4, 50, seed=1).requires_grad_(True), randn(9, 6, seed=2).requires_grad_(True)
+    y = some_tokens(4, 50, 3)
+    for out, leaf in ((learn.logprobs(x, y).entropy.sum(), x),
+                      (learn.embedding(y.clamp(max=8), w).square().sum(), w)):
+        g, = torch.autograd.grad(out, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
+
+
+def test_inputs_changed_in_place_are_seen():
+    x, y = randn(4, 50, seed=1), some_tokens(4, 50, 3)
+    leaf = x.clone().requires_grad_(True)
+    moved = leaf * 1.0
+    out = learn.logprobs(moved, y).logprob.sum()
+    with torch.no_grad():
+        moved.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        out.backward()
+    t = torch.tensor([1, 2], device="cuda")
+    rows = learn.embedding(t, randn(5, 3, seed=1).requires_grad_(True)).sum()
+    t.zero_()
+    with pytest.raises(RuntimeError):
+        rows.backward()
