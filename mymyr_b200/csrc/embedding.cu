@@ -138,7 +138,7 @@ constexpr size_t cluster_bytes(u32 share)
 __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const Tokens in, u32 n, u32 share, u32 passes, u32 bits,
                                                                   u32* __restrict__ keys, u32* __restrict__ places,
                                                                   u32* __restrict__ held_count, u32* __restrict__ joins,
-                                                                  u32* __restrict__ long_joins, const Zeros zeros)
+                                                                  const Zeros zeros)
 {
     const u32 t = threadIdx.x, lane = t & 31, w = t >> 5;
     if (blockIdx.x >= kClusterBlocks)
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const Tokens i
     if (q == 0 && t == 0)
     {
         *held_count = total;
-        joins[0] = long_joins[0] = 0;
+        *joins = 0;
     }
 }
 
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kBins) k_sort_scan(u32* __restrict__ counts, u
 __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Pass in, const u32* __restrict__ counts,
                                                              const u32* __restrict__ totals, u32* __restrict__ keys,
                                                              u32* __restrict__ places, u32* __restrict__ held_count,
-                                                             u32* __restrict__ joins, u32* __restrict__ long_joins)
+                                                             u32* __restrict__ joins)
 {
     __shared__ u32 at[kSortBlock / 32][kBins];
     __shared__ u32 tmp[kBins / 32], first[kBins], shift_to[kBins];
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const Pass in, cons
     if (held_count && blockIdx.x == 0 && threadIdx.x == 0)
     {
         *held_count = all;
-        joins[0] = long_joins[0] = 0;
+        *joins = 0;
     }
     __syncthreads();
 #pragma unroll
@@ -411,8 +411,7 @@ struct Segments
     float scale;
     u64 width, grad_stride;
     float* partial;  // [chunks, 2, width]: of the token that comes into the chunk, of the one that goes on after it
-    u32* joins;       // the number of chunks out of which a token goes on that did not come into them, and these chunks
-    u32* long_joins;  // of them, those whose token comes into many chunks
+    u32* joins;      // the number of chunks out of which a token goes on that did not come into them, and these chunks
 };
 
 template<class T, int VE>
@@ -496,83 +495,97 @@ __global__ void __launch_bounds__(256) k_segment_sum(const Segments a, const T* 
 
 constexpr u32 kJoinColumns = 128, kJoinShort = 16;
 
-/// Joins the partial sums of each token that crosses a few chunks, a warp for a token and 128 columns; a token of more
-/// chunks goes to the list of the long ones.
+/// Joins the partial sums of each token that crosses chunks: a warp for a token and 128 columns where the token lies in
+/// few chunks; where it lies in many, the warps of the block that met it take every eighth chunk each, and their sums
+/// are added in the warps' order. The order of a sum depends on its chunks alone, not on who takes it. Bound by some six
+/// dependent loads (6 us).
 template<class T>
 __global__ void __launch_bounds__(256) k_segment_join(const Segments a, T* __restrict__ out, u32 slices)
 {
-    const u32 n = *a.count, lane = threadIdx.x & 31;
-    const u64 items = static_cast<u64>(a.joins[0]) * slices;
-    for (u64 item = (static_cast<u64>(blockIdx.x) * 256 + threadIdx.x) / 32; item < items; item += gridDim.x * 8ull)
-    {
-        const u32 c = a.joins[1 + item / slices], slice = static_cast<u32>(item % slices);
-        const u32 key = a.keys[static_cast<u64>(c + 1) * a.chunk];
-        const u64 first = (static_cast<u64>(c) + 1 + lane) * a.chunk;
-        const u32 span = __popc(__ballot_sync(~0u, first < n && a.keys[first] == key));  // chunks that it comes into
-        if (span > kJoinShort)
-        {
-            if (slice == 0 && lane == 0)
-                a.long_joins[1 + atomicAdd(a.long_joins, 1u)] = c;
-            continue;
-        }
-        const u64 column = static_cast<u64>(slice) * kJoinColumns + lane;
-        const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
-        float sum[kJoinColumns / 32] = {};
-#pragma unroll 4
-        for (u32 i = 0; i <= span; ++i)
-        {
-            // the first partial sum is of the token that goes on, the others of the one that comes in
-#pragma unroll
-            for (u32 k = 0; k < kJoinColumns / 32; ++k)
-                if (column + k * 32 < a.width)
-                    sum[k] += from[(static_cast<u64>(i) * 2 + (i == 0)) * a.width + k * 32];
-        }
+    __shared__ float sums[8][kJoinColumns];
+    __shared__ u32 long_items[8], long_count;
+    const u32 n = *a.count, lane = threadIdx.x & 31, w = threadIdx.x >> 5, joins = a.joins[0];
+    const u64 items = static_cast<u64>(joins) * slices;
+    if (threadIdx.x == 0)
+        long_count = 0;
+    __syncthreads();
+    // the first partial sum is of the token that goes on, the others of the one that comes in
+    auto add = [&](float(&sum)[kJoinColumns / 32], const float* from, u32 i, u64 column) {
 #pragma unroll
         for (u32 k = 0; k < kJoinColumns / 32; ++k)
             if (column + k * 32 < a.width)
-                out[key * a.width + column + k * 32] = from_f32<T>(sum[k] * a.scale);
-    }
-}
-
-/// Those of many chunks, a block for a token and `lanes` columns (a power of two up to 32): 256 / lanes rows of threads
-/// over the chunks, whose sums are added as a tree.
-template<class T>
-__global__ void __launch_bounds__(256) k_segment_join_long(const Segments a, T* __restrict__ out, u32 lanes, u32 slices)
-{
-    __shared__ float sums[256];
-    const u32 n = *a.count, rows = 256 / lanes, row = threadIdx.x / lanes;
-    const u64 items = static_cast<u64>(a.long_joins[0]) * slices;
-    for (u64 item = blockIdx.x; item < items; item += gridDim.x)
+                sum[k] += from[(static_cast<u64>(i) * 2 + (i == 0)) * a.width + k * 32];
+    };
+    // an item for each block before a block has two: long ones take all of it
+    for (u64 group = blockIdx.x; group < items; group += gridDim.x * 8ull)
     {
-        const u32 c = a.long_joins[1 + item / slices], key = a.keys[static_cast<u64>(c + 1) * a.chunk];
-        const u64 column = item % slices * lanes + (threadIdx.x & (lanes - 1));
-        u32 more = 1;
-        for (;;)
+        const u64 item = group + w * gridDim.x;
+        if (item < items)
         {
-            const u64 first = (static_cast<u64>(c) + 1 + more + threadIdx.x) * a.chunk;
-            const u32 got = __syncthreads_count(first < n && a.keys[first] == key);
-            more += got;
-            if (got < blockDim.x)
-                break;
+            const u32 slice = static_cast<u32>(item / joins);
+            const u32 c = a.joins[1 + item - static_cast<u64>(slice) * joins];
+            const u32 key = a.keys[static_cast<u64>(c + 1) * a.chunk];
+            const u64 first = (static_cast<u64>(c) + 1 + lane) * a.chunk;
+            const u32 span = __popc(__ballot_sync(~0u, first < n && a.keys[first] == key));  // chunks that it comes into
+            const u64 column = static_cast<u64>(slice) * kJoinColumns + lane;
+            if (span > kJoinShort)
+            {
+                if (lane == 0)
+                    long_items[atomicAdd(&long_count, 1u)] = w;
+            }
+            else
+            {
+                const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
+                float sum[kJoinColumns / 32] = {};
+#pragma unroll 4
+                for (u32 i = 0; i <= span; ++i)
+                    add(sum, from, i, column);
+#pragma unroll
+                for (u32 k = 0; k < kJoinColumns / 32; ++k)
+                    if (column + k * 32 < a.width)
+                        out[key * a.width + column + k * 32] = from_f32<T>(sum[k] * a.scale);
+            }
         }
-        float sum = 0.f;
-        if (column < a.width)
-        {
-            const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
-#pragma unroll 8
-            for (u32 i = row; i <= more; i += rows)
-                sum += from[(static_cast<u64>(i) * 2 + (i == 0)) * a.width];
-        }
-        sums[threadIdx.x] = sum;
         __syncthreads();
-        for (u32 half = rows / 2; half; half /= 2)
+        const u32 many = long_count;
+        for (u32 l = 0; l < many; ++l)
         {
-            if (row < half)
-                sums[threadIdx.x] += sums[threadIdx.x + half * lanes];
+            const u64 which = group + long_items[l] * gridDim.x;
+            const u32 slice = static_cast<u32>(which / joins);
+            const u32 c = a.joins[1 + which - static_cast<u64>(slice) * joins];
+            const u32 key = a.keys[static_cast<u64>(c + 1) * a.chunk];
+            u32 more = kJoinShort;
+            for (;;)
+            {
+                const u64 first = (static_cast<u64>(c) + 1 + more + threadIdx.x) * a.chunk;
+                const u32 got = __syncthreads_count(first < n && a.keys[first] == key);
+                more += got;
+                if (got < blockDim.x)
+                    break;
+            }
+            const u64 column = static_cast<u64>(slice) * kJoinColumns + lane;
+            const float* const from = a.partial + static_cast<u64>(c) * 2 * a.width + column;
+            float sum[kJoinColumns / 32] = {};
+#pragma unroll 8
+            for (u32 i = w; i <= more; i += 8)
+                add(sum, from, i, column);
+#pragma unroll
+            for (u32 k = 0; k < kJoinColumns / 32; ++k)
+                sums[w][k * 32 + lane] = sum[k];
+            __syncthreads();
+            const u64 mine = static_cast<u64>(slice) * kJoinColumns + threadIdx.x;
+            if (threadIdx.x < kJoinColumns && mine < a.width)
+            {
+                float all = 0.f;
+#pragma unroll
+                for (u32 i = 0; i < 8; ++i)
+                    all += sums[i][threadIdx.x];
+                out[key * a.width + mine] = from_f32<T>(all * a.scale);
+            }
             __syncthreads();
         }
-        if (row == 0 && column < a.width)
-            out[key * a.width + column] = from_f32<T>(sums[threadIdx.x] * a.scale);
+        if (many && threadIdx.x == 0)
+            long_count = 0;
         __syncthreads();
     }
 }
@@ -646,7 +659,7 @@ struct Plan
 {
     u32 n, passes, bits, tiles, chunk, chunks;
     bool cluster;
-    size_t keys[2], places[2], counts, totals, held, joins, long_joins, partial, bytes;
+    size_t keys[2], places[2], counts, totals, held, joins, partial, bytes;
 };
 
 Plan plan_of(const b2_embedding_args& a)
@@ -687,7 +700,6 @@ Plan plan_of(const b2_embedding_args& a)
     }
     p.held = take(4);
     p.joins = take((static_cast<size_t>(p.chunks) + 1) * 4);
-    p.long_joins = take((static_cast<size_t>(p.chunks) + 1) * 4);
     p.partial = take(static_cast<size_t>(p.chunks) * 2 * a.width * 4);
     p.bytes = at;
     return p;
@@ -703,7 +715,6 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
     const u64 vectors = zeros.bytes / 32 + 1;
     s.count = words(p.held);
     s.joins = words(p.joins);
-    s.long_joins = words(p.long_joins);
     if (p.cluster)
     {
         const u32 share = std::max(1u, (p.n + kClusterBlocks * kClusterThreads - 1) / (kClusterBlocks * kClusterThreads)) *
@@ -732,7 +743,7 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
         s.keys = words(p.keys[0]);
         s.places = words(p.places[0]);
         B2_CUDA(cudaLaunchKernelEx(&cfg, k_sort_cluster, tokens, p.n, share, p.passes, p.bits, words(p.keys[0]),
-                                   words(p.places[0]), words(p.held), words(p.joins), words(p.long_joins), zeros));
+                                   words(p.places[0]), words(p.held), words(p.joins), zeros));
         return;
     }
     Pass in{tokens, nullptr, nullptr, nullptr, p.n, 0, p.bits, p.tiles};
@@ -745,8 +756,7 @@ void sort_tokens(const b2_ctx& ctx, const b2_embedding_args& a, const Plan& p, c
         k_sort_count<<<p.tiles + extra, kSortBlock, 0, st>>>(in, words(p.counts), zeros);
         k_sort_scan<<<1u << p.bits, kBins, 0, st>>>(words(p.counts), p.tiles, words(p.totals));
         k_sort_scatter<<<p.tiles, kSortBlock, 0, st>>>(in, words(p.counts), words(p.totals), keys, places,
-                                                       i == 0 ? words(p.held) : nullptr, words(p.joins),
-                                                       words(p.long_joins));
+                                                       i == 0 ? words(p.held) : nullptr, words(p.joins));
         in.keys = s.keys = keys;
         in.places = s.places = places;
         in.count = s.count;
@@ -855,20 +865,10 @@ b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, cons
             });
             if (s.chunks > 1)
             {
-                u32 slices = static_cast<u32>((a.width + kJoinColumns - 1) / kJoinColumns);
+                const u32 slices = static_cast<u32>((a.width + kJoinColumns - 1) / kJoinColumns);
                 const u64 warps = static_cast<u64>(s.chunks) * slices;
-                T* const out = static_cast<T*>(grad_weight);
-                k_segment_join<T><<<grid_for(warps, 8, static_cast<unsigned>(ctx->sms) * 8), 256, 0, st>>>(s, out, slices);
-                if (s.chunks > kJoinShort + 1)
-                {
-                    u32 lanes = 1;
-                    while (lanes < 32 && lanes < a.width)
-                        lanes *= 2;
-                    slices = static_cast<u32>((a.width + lanes - 1) / lanes);
-                    const u64 blocks = static_cast<u64>(s.chunks) / (kJoinShort + 1) * slices;
-                    k_segment_join_long<T><<<grid_for(blocks, 1, static_cast<unsigned>(ctx->sms) * 4), 256, 0, st>>>(
-                        s, out, lanes, slices);
-                }
+                k_segment_join<T><<<grid_for(warps, 1, static_cast<unsigned>(ctx->sms) * 8), 256, 0, st>>>(
+                    s, static_cast<T*>(grad_weight), slices);
             }
             B2_CUDA(cudaGetLastError());
         });
