@@ -185,14 +185,14 @@ __device__ __forceinline__ float above_least(float x)
 /// just advance between them.
 ///
 /// Bound by HBM in 32 bits: 28 bytes for an element (parameter, gradient and moments read, all but the gradient written),
-/// 174 M bf16 parameters with masters in 758 us (6.4 TB/s). With 8-bit moments it is 10 bytes and some 65 instructions,
-/// and these bound it: 329 M parameters in 750 us (4.4 TB/s); five blocks an SM against four, runs of blocks and codes
-/// from the square root alone brought it from 854, fetching the next block ahead or all arithmetic in pairs took it back
-/// (fewer warps, more moves). One pass: everything of an element is in registers between its loads and its stores, the
+/// 174 M bf16 parameters with masters in 748 us (6.5 TB/s). With 8-bit moments it is 10 bytes and some 60 instructions,
+/// and these bound it: 329 M parameters in 682 us (4.9 TB/s). Five or three blocks an SM, fetching the next block ahead,
+/// taking elements in pairs or all arithmetic packed in pairs measured slower (registers, moves). One pass: everything of
+/// an element is in registers between its loads and its stores, the
 /// block's largest magnitudes come from the warp's 32-bit maximum reduction. Averages are separate multiplications and
 /// additions (not fused): the scales and codes then are those of the formula as written, on any machine.
 template<class P, class G, int BITS, bool MASTER, u32 N>
-__global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
+__global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
                                                        u32 key, u32 run)
 {
     using M = std::conditional_t<BITS == 8, uint8_t, float>;
@@ -238,142 +238,148 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 8 ? 5 : 4) k_adamw(const 
         M* const m_at = static_cast<M*>(s.m) + at;
         M* const v_at = static_cast<M*>(s.v) + at;
         float* const master = s.master + at;
-        // a tensor's last block, and tensors that start off a vector's boundary, go element by element
         const u32 n = static_cast<u32>(min(left, static_cast<u64>(kMoment)));
-        const bool whole = aligned && n == kMoment;
-        float gi[8], now[8], m[8], v[8], r[8];
-        if (whole)
-        {
-            load8(g, gi);
-            if (!MASTER)
-                load8(p, now);
-        }
-        else
-        {
-#pragma unroll
-            for (u32 k = 0; k < 8; ++k)
+        auto body = [&]<bool whole>() {
+            float gi[8], now[8], m[8], v[8], r[8];
+            if (whole)
             {
-                gi[k] = i0 + k < n ? to_f32(g[k]) : 0.f;
+                load8(g, gi);
                 if (!MASTER)
-                    now[k] = i0 + k < n ? to_f32(p[k]) : 0.f;
+                    load8(p, now);
             }
-        }
-        if constexpr (MASTER)
-            load8(master, now);
-        if constexpr (BITS == 8)
-        {
-            decode8(*reinterpret_cast<const uint2*>(m_at), m);
-            decode8(*reinterpret_cast<const uint2*>(v_at), r);
-            const float ms = s.m_scale[block], vs = s.v_scale[block];
-            const Two ms2(ms, ms), vs2(vs, vs);
-#pragma unroll
-            for (int k = 0; k < 8; k += 2)
+            else
             {
-                const float2 x = (Two(m[k], m[k + 1]) * ms2).get();
-                const Two y = Two(r[k], r[k + 1]) * vs2;
-                const float2 z = (y * y).get();
-                m[k] = x.x, m[k + 1] = x.y, v[k] = z.x, v[k + 1] = z.y;
-            }
-        }
-        else
-        {
-            load8(m_at, m);
-            load8(v_at, v);
-        }
 #pragma unroll
-        for (int k = 0; k < 8; k += 2)
-        {
-            const Two g2(gi[k], gi[k + 1]);
-            const float2 x = fma(Two(m[k], m[k + 1]) * b1, one, g2 * a1).get();
-            const float2 y = fma(Two(v[k], v[k + 1]) * b2, one, g2 * g2 * a2).get();
-            m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
-        }
-        float m_most = 0.f, v_most = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-        {
-            // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
-            float floor;
-            asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
-            float rest;
-            const float root = sqrt_fast(floor, rest);
-            // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
-            r[k] = BITS == 8 ? root + rest : root;
-            now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
-            if constexpr (BITS == 8)
-            {
-                m_most = max_magnitude(m_most, m[k]);
-                v_most = max_magnitude(v_most, v[k]);
-            }
-        }
-        if constexpr (MASTER)
-            store8(master, now);
-        if (whole)
-            store8(p, now);
-        else
-        {
-#pragma unroll
-            for (u32 k = 0; k < 8; ++k)
-                if (i0 + k < n)
-                    p[k] = from_f32<P>(now[k]);
-        }
-        if constexpr (BITS == 32)
-        {
-            store8(m_at, m);
-            store8(v_at, v);
-        }
-        else
-        {
-            u32 top = largest_of(m_most, m);
-            bool bad = top >> 31;
-            const float ms = scale_of(top), mi = inverse_power(ms);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                m[k] *= mi;
-            if (bad)  // an infinity becomes NaN as NaN does, not the largest code
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    m[k] = m[k] - m[k] == 0.f ? m[k] : nanf("");
-            *reinterpret_cast<uint2*>(m_at) = encode8(m);
-            // the square root of the largest is the largest square root
-            top = __reduce_max_sync(~0u, __float_as_uint(v_most));
-            bad = top >= kInfBits;
-            top = bad ? largest_of(__uint_as_float(top), r) : __float_as_uint(__fsqrt_rn(__uint_as_float(top)));
-            const float vs = scale_of(top);
-            const u32 vs_exponent = __float_as_uint(vs) - (127u << 23);
-            const u32 pair = block * (kMoment / 2) + i0 / 2;  // of the element among all, modulo 2^32
-            float code[8];
-#pragma unroll
-            for (int k = 0; k < 8; k += 2)
-            {
-                const u32 bits = mix((pair + k / 2) ^ key);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (u32 k = 0; k < 8; ++k)
                 {
-                    // u = (16 bits + 1/2) / 2^16 as the number 1 + u
-                    const u32 part = j ? bits >> 9 : bits << 7;
-                    const float u1 = __uint_as_float(0x3F800040u | (part & 0x7FFF80u));
-                    // r / (unit scale) is in [8, 16), or below 8 among the smallest codes; its floor, by way of 2^23
-                    const u32 ex = max(__float_as_uint(r[k + j]) & kInfBits, (121u << 23) + vs_exponent);
-                    const float q = r[k + j] * __uint_as_float((257u << 23) - ex);
-                    const float low = __fadd_rd(q, 0x1p23f) - 0x1p23f;
-                    // up with the probability that keeps the square's mean: (q^2 - low^2) / ((low + 1)^2 - low^2)
-                    const float step = fmaf(2.f, low, 1.f), edge = fmaf(u1, step, fmaf(low, low, -step));
-                    const float up = q * q > edge ? low + 1.f : low;
-                    code[k + j] = fmaxf(up, above_least(r[k + j])) * __uint_as_float(ex - (3u << 23) - vs_exponent);
+                    gi[k] = i0 + k < n ? to_f32(g[k]) : 0.f;
+                    if (!MASTER)
+                        now[k] = i0 + k < n ? to_f32(p[k]) : 0.f;
                 }
             }
-            if (bad)
+            if constexpr (MASTER)
+                load8(master, now);
+            if constexpr (BITS == 8)
+            {
+                decode8(*reinterpret_cast<const uint2*>(m_at), m);
+                decode8(*reinterpret_cast<const uint2*>(v_at), r);
+                const float ms = s.m_scale[block], vs = s.v_scale[block];
+                const Two ms2(ms, ms), vs2(vs, vs);
+#pragma unroll
+                for (int k = 0; k < 8; k += 2)
+                {
+                    const float2 x = (Two(m[k], m[k + 1]) * ms2).get();
+                    const Two y = Two(r[k], r[k + 1]) * vs2;
+                    const float2 z = (y * y).get();
+                    m[k] = x.x, m[k + 1] = x.y, v[k] = z.x, v[k + 1] = z.y;
+                }
+            }
+            else
+            {
+                load8(m_at, m);
+                load8(v_at, v);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k += 2)
+            {
+                const Two g2(gi[k], gi[k + 1]);
+                const float2 x = fma(Two(m[k], m[k + 1]) * b1, one, g2 * a1).get();
+                const float2 y = fma(Two(v[k], v[k + 1]) * b2, one, g2 * g2 * a2).get();
+                m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
+            }
+            [[maybe_unused]] float m_most = 0.f, v_most = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+            {
+                // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
+                float floor;
+                asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
+                float rest;
+                const float root = sqrt_fast(floor, rest);
+                // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
+                r[k] = BITS == 8 ? root + rest : root;
+                now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
+                if constexpr (BITS == 8)
+                {
+                    m_most = max_magnitude(m_most, m[k]);
+                    v_most = max_magnitude(v_most, v[k]);
+                }
+            }
+            if constexpr (MASTER)
+                store8(master, now);
+            if (whole)
+                store8(p, now);
+            else
+            {
+#pragma unroll
+                for (u32 k = 0; k < 8; ++k)
+                    if (i0 + k < n)
+                        p[k] = from_f32<P>(now[k]);
+            }
+            if constexpr (BITS == 32)
+            {
+                store8(m_at, m);
+                store8(v_at, v);
+            }
+            else
+            {
+                u32 top = largest_of(m_most, m);
+                bool bad = top >> 31;
+                const float ms = scale_of(top), mi = inverse_power(ms);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    code[k] = r[k] - r[k] == 0.f ? code[k] : nanf("");
-            *reinterpret_cast<uint2*>(v_at) = encode8(code);
-            if (lane == 0)
-            {
-                s.m_scale[block] = ms;
-                s.v_scale[block] = vs;
+                    m[k] *= mi;
+                if (bad)  // an infinity becomes NaN as NaN does, not the largest code
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        m[k] = m[k] - m[k] == 0.f ? m[k] : nanf("");
+                *reinterpret_cast<uint2*>(m_at) = encode8(m);
+                // the square root of the largest is the largest square root
+                top = __reduce_max_sync(~0u, __float_as_uint(v_most));
+                bad = top >= kInfBits;
+                top = bad ? largest_of(__uint_as_float(top), r) : __float_as_uint(__fsqrt_rn(__uint_as_float(top)));
+                const float vs = scale_of(top);
+                const u32 vs_exponent = __float_as_uint(vs) - (127u << 23);
+                const u32 pair = block * (kMoment / 2) + i0 / 2;  // of the element among all, modulo 2^32
+                float code[8];
+#pragma unroll
+                for (int k = 0; k < 8; k += 2)
+                {
+                    const u32 bits = mix((pair + k / 2) ^ key);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                    {
+                        // u = (16 bits + 1/2) / 2^16 as the number 1 + u
+                        const u32 part = j ? bits >> 9 : bits << 7;
+                        const float u1 = __uint_as_float(0x3F800040u | (part & 0x7FFF80u));
+                        // r / (unit scale) is in [8, 16), or below 8 among the smallest codes; its floor, by way of 2^23
+                        const u32 ex = max(__float_as_uint(r[k + j]) & kInfBits, (121u << 23) + vs_exponent);
+                        const float q = r[k + j] * __uint_as_float((257u << 23) - ex);
+                        const float low = __fadd_rd(q, 0x1p23f) - 0x1p23f;
+                        // up with the probability that keeps the square's mean: (q^2 - low^2) / ((low + 1)^2 - low^2)
+                        const float step = fmaf(2.f, low, 1.f), edge = fmaf(u1, step, fmaf(low, low, -step));
+                        const float up = q * q > edge ? low + 1.f : low;
+                        code[k + j] = fmaxf(up, above_least(r[k + j])) * __uint_as_float(ex - (3u << 23) - vs_exponent);
+                    }
+                }
+                if (bad)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        code[k] = r[k] - r[k] == 0.f ? code[k] : nanf("");
+                *reinterpret_cast<uint2*>(v_at) = encode8(code);
+                if (lane == 0)
+                {
+                    s.m_scale[block] = ms;
+                    s.v_scale[block] = vs;
+                }
             }
-        }
+        };
+        // a tensor's last block, and tensors that start off a vector's boundary, go element by element (a body of their own:
+        // together with the others' it cost 10 %)
+        if (aligned && n == kMoment)
+            body.template operator()<true>();
+        else
+            body.template operator()<false>();
         p += kMoment, g += kMoment, at += kMoment;
         left -= n, ++block;
     }
@@ -394,8 +400,8 @@ void launch(const b2_ctx& ctx, const b2_adamw_args& a, u32 first, u32 count, con
     t.blocks = static_cast<u32>(blocks);
     const u32 key = mix(mix(a.seed) ^ static_cast<u32>(a.step));
     const Moments s{a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.master};
-    // runs of up to 32 blocks, while the warps that the device holds have four each
-    const u32 run = static_cast<u32>(std::min<u64>(32, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 128))));
+    // runs of up to 8 blocks, 32 of 8-bit moments (730 us with 8), while the warps that the device holds have four each
+    const u32 run = static_cast<u32>(std::min<u64>(BITS == 8 ? 32 : 8, std::max<u64>(1, blocks / (static_cast<u64>(ctx.sms) * 128))));
     const u64 per = static_cast<u64>(kWarps) * run;
     k_adamw<P, G, BITS, MASTER, N>
         <<<static_cast<unsigned>((blocks + per - 1) / per), kWarps * 32, 0, st>>>(t, s, h, key, run);
