@@ -969,7 +969,8 @@ enum class Layout
 
 /// By the mean length. Few lanes with many logits each cost less than many with few: most of a short row's instructions
 /// are its sums over the lanes and its results (65,536 rows of 100 bf16: 16 us forward, with 32 lanes 41). A warp takes
-/// vectors, 32 at a time, while a row has few or the rows fill the device with warps.
+/// vectors, 32 at a time, while a row has few or there are rows enough (with gradient, warps and blocks: 30,000 rows of
+/// 2,000 bf16 85 and 152 us, 6,000 of 4,000 36 and 44, 16,384 of 8,000 153 and 166, 2,400 of 8,000 32 and 28).
 template<class T>
 Layout layout_of(const b2_ctx& ctx, const Rows& rows, u64 count)
 {
@@ -978,7 +979,9 @@ Layout layout_of(const b2_ctx& ctx, const Rows& rows, u64 count)
         return Layout::lanes4;
     if (mean <= 128)
         return Layout::lanes8;
-    return vectors <= 256 || (vectors <= 1024 && count >= static_cast<u64>(ctx.sms) * 16) ? Layout::warp : Layout::block;
+    const u64 full = static_cast<u64>(ctx.sms) * 16;  // half of the warps that the device holds
+    return vectors <= 256 || (vectors <= 512 && count >= full) || (vectors <= 1024 && count >= 5 * full) ? Layout::warp
+                                                                                                      : Layout::block;
 }
 
 template<class T, bool MASK, bool TOP, int NW, int U, int ROWS>
@@ -1028,8 +1031,8 @@ void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
     // enough to make up for what a larger block waits for at their ends (16,384 rows of 15,000 bf16: 102 us, with 8 warps
     // 134; 2,048 of 50,001 fp32 with 8 alternatives: 106 and 84), nor many alternatives to be looked for among few
     // threads' logits (16,384 of 30,001 bf16 with 20: 344 and 314)
-    const bool few_warps = f.count >= static_cast<u64>(ctx.sms) * 8 && f.top <= 8 &&
-                           mean <= (f.top ? 4096u : 8192u) * kVec<T>;
+    const bool few_warps = f.top <= 8 && mean <= (f.top ? 4096u : 8192u) * kVec<T> &&
+                           f.count >= static_cast<u64>(ctx.sms) * (mean <= 2048 * kVec<T> ? 8 : 40);
     with_flags([&]<bool MASK, bool TOP>() {
         if (cluster > 1)
             forward_long<T, MASK, TOP, NW, 8, 1>(f, cluster, st);
