@@ -1,5 +1,4 @@
 // Log-probabilities of given tokens with entropy and the best alternatives, and the gradient of the logits.
-
 //
 // One pass over a row's logits x: with a reference r, S = sum 2^d and T = sum 2^d d for d = (x - r) log2(e) / temperature
 // give log-probabilities (x - r) / temperature - ln S and the entropy ln 2 (log2 S - T / S); partial sums of other
@@ -7,9 +6,9 @@
 // the logits that it read, the k best threads hold the k best logits, and only their logits are read again (from cache).
 //
 // Bound by HBM where rows are long and many, by the latency of a few dependent steps where they are few, and by
-// instruction issue where they are short. So rows are laid out by their length: a group of 4, 8 or 32 lanes for a
-// short row, a block for a long one, a cluster of blocks (joined over distributed shared memory) where long rows are
-// too few to fill the device.
+// instruction issue where they are short. So rows are laid out by their length and number: a group of 4 or 8 lanes for a
+// short row, a warp for a middling one, a block for a long one, a cluster of blocks (joined over distributed shared
+// memory) where long rows are too few to fill the device.
 
 #include "learn.cuh"
 
@@ -955,7 +954,7 @@ Rows rows_of(const b2_logprobs_args& a)
     return {a.logits, a.offsets, a.mask, a.row_stride, a.mask_stride, a.width, a.offsets_bits};
 }
 
-/// The mean length of a call's rows, by which they are laid out (ragged rows that are longer still are right, if slower).
+/// The mean length of a call's rows, by which they are laid out (ragged rows that are much longer are right, if slower).
 u64 mean_length(const Rows& rows, u64 count) { return rows.offsets ? rows.width / count : rows.width; }
 
 /// How a call's rows are laid out.
