@@ -503,11 +503,12 @@ typedef struct b2_adamw_args {
     int32_t grad_dtype;      /* param_dtype or B2_F32 */
     int32_t moment_bits;     /* 32: float moments; 8: float8 e4m3 codes with a scale for each block */
     uint64_t blocks;         /* of the moment arrays */
-    void* exp_avg;           /* [blocks * 256] */
-    void* exp_avg_sq;        /* [blocks * 256]; 8 bits: the codes of the second moment's square root */
+    void* exp_avg;           /* [blocks * 256]; aligned to eight elements: 32 bytes, 8 bits: 8 bytes */
+    void* exp_avg_sq;        /* as exp_avg; 8 bits: the codes of the second moment's square root */
     float* exp_avg_scale;    /* [blocks], 8 bits */
     float* exp_avg_sq_scale; /* [blocks], 8 bits */
-    float* master;           /* [blocks * 256] 32-bit parameters the 16-bit ones are rounded from, or NULL */
+    float* master;           /* [blocks * 256], 32-byte aligned: the 32-bit parameters that the 16-bit ones are
+                                rounded from; or NULL */
     double lr, beta1, beta2, eps, weight_decay;
     uint64_t step;           /* of this update, from 1 */
     uint32_t seed;           /* 8 bits: of the second moment's rounding */

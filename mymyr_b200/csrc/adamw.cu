@@ -470,6 +470,11 @@ extern "C" b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stre
             throw bad("more than 2^32 - 1 blocks of work");
         if (!a.exp_avg || !a.exp_avg_sq || (a.moment_bits == 8 && (!a.exp_avg_scale || !a.exp_avg_sq_scale)))
             throw bad("null moments");
+        // what the kernel takes eight elements at a time of, whole blocks or not
+        auto aligned = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+        const uintptr_t unit = a.moment_bits;  // eight moments, in bytes
+        if (!aligned(a.exp_avg, unit) || !aligned(a.exp_avg_sq, unit) || !aligned(a.master, 32))
+            throw bad("moments and master must start on a boundary of eight elements (32 bytes, 8 for 8-bit moments)");
         const OnDevice on(ctx->device);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         dispatch_dtype(a.param_dtype, "b2_adamw", [&]<class P>() {

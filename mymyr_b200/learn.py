@@ -137,6 +137,7 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p = p (1 - lr weight_decay) - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)
 
+    Moments of another origin (a part of a larger buffer) must be contiguous and start on a boundary of eight elements.
     A gradient is of its parameter's type or float32; one that is None leaves its tensor alone. Parameters of 16 bits
     are rounded to nearest from ``master`` if given. 8-bit moments are rounded for storage only: the first to nearest,
     the second to one of its two neighbours by random numbers of (``seed``, step, element), so that the small steps of
