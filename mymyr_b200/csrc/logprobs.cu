@@ -1086,6 +1086,8 @@ void check_args(b2_ctx* ctx, const b2_logprobs_args* a, const char* what)
         throw bad("temperature must be positive and finite, and its inverse too");
     if (a->top > B2_TOP_MAX)
         throw bad("more than 32 alternatives");
+    if (reinterpret_cast<uintptr_t>(a->stats) % 16)
+        throw bad("stats must be 16-byte aligned");
 }
 }  // namespace
 }  // namespace b2

@@ -29,6 +29,38 @@ def randn(*shape, seed=0, scale=1.0):
     return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") * scale
 
 
+# ------------------------------------------------------------------------------------------------ log-probabilities
+
+def c_logprobs(logits, tokens=None, **more):
+    """The C ABI's arguments for dense rows; the tensors must outlive them."""
+    a = _lib.LogprobsArgs()
+    a.logits, a.dtype = logits.data_ptr(), [torch.float32, torch.bfloat16, torch.float16].index(logits.dtype)
+    a.rows, a.width, a.row_stride, a.temperature = *logits.shape, logits.stride(0), 1.0
+    if tokens is not None:
+        a.tokens, a.token_bits = tokens.data_ptr(), 64
+    for k, v in more.items():
+        setattr(a, k, v.data_ptr() if isinstance(v, torch.Tensor) else v)
+    return a
+
+
+def test_statistics_off_a_16_byte_boundary_are_refused():
+    """By the host, before anything is launched."""
+    L, h = _lib.lib(), default_context().handle
+    x, out, stats = randn(3, 9, seed=1), torch.zeros(3, device="cuda"), torch.zeros(16, device="cuda")
+    grad = torch.full_like(x, 7.0)
+    for off in (1, 2, 3):
+        a = c_logprobs(x, entropy=out, stats=stats[off:])
+        assert L.b2_logprobs(h, C.byref(a), None) == _lib.B2_INVALID_ARGUMENT
+        assert L.b2_logprobs_backward(h, C.byref(a), None, out.data_ptr(), grad.data_ptr(), 9,
+                                      None) == _lib.B2_INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    assert (out == 0).all() and (grad == 7).all()
+    a = c_logprobs(x, entropy=out, stats=stats[4:])
+    assert L.b2_logprobs(h, C.byref(a), None) == 0
+    torch.cuda.synchronize()
+    assert (out > 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ AdamW
 
 def shifted(t, by):
