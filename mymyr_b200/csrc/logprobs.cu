@@ -1122,12 +1122,17 @@ b2_status b2_logprobs_backward(b2_ctx* ctx, const b2_logprobs_args* args, const 
     return guarded([&] {
         check_args(ctx, args, "b2_logprobs_backward");
         const b2_logprobs_args& a = *args;
-        if (a.rows && (!a.stats || (a.width && !grad_logits)))
+        if ((a.rows && !a.stats) || (a.width && (a.rows || a.offsets) && !grad_logits))
             throw std::invalid_argument("b2_logprobs_backward: null stats or output");
         dispatch_dtype(a.dtype, "b2_logprobs_backward", [&]<class T>() {
-            if (!a.rows || !a.width)
+            if (!a.width || !(a.rows || a.offsets))
                 return;
             const OnDevice on(ctx->device);
+            if (!a.rows)  // a vector without rows: none of it takes part
+            {
+                B2_CUDA(cudaMemsetAsync(grad_logits, 0, a.width * sizeof(T), static_cast<cudaStream_t>(stream)));
+                return;
+            }
             const Backward f{rows_of(a), a.rows, a.tokens, a.token_bits, 1, 1.f / a.temperature, a.stats,
                              a.tokens ? grad_logprob : nullptr, grad_entropy, grad_logits, grad_stride};
             backward<T>(*ctx, f, static_cast<cudaStream_t>(stream));

@@ -61,6 +61,21 @@ def test_statistics_off_a_16_byte_boundary_are_refused():
     assert (out > 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("first", [0, 17])
+def test_gradient_of_a_vector_without_rows(dtype, first):
+    """One offset, so no rows, over a buffer of logits: the gradient is zero all over, not what the memory held."""
+    offsets = torch.tensor([first], device="cuda")
+    for n in (1, 60, 5001):
+        leaf = randn(n, seed=n).to(dtype).requires_grad_(True)
+        got = learn.logprobs(leaf, torch.zeros(0, dtype=torch.int64, device="cuda"), offsets=offsets, top=2)
+        assert got.entropy.shape == got.logprob.shape == (0,) and got.top_tokens.shape == (0, 2)
+        held = torch.full_like(leaf, float("nan"))  # what the allocator is to hand out again
+        del held
+        g, = torch.autograd.grad(got.entropy.sum() + got.logprob.sum(), leaf)
+        assert g.shape == leaf.shape and (g == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ AdamW
 
 def shifted(t, by):
