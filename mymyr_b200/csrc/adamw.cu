@@ -144,6 +144,7 @@ __device__ __forceinline__ float max_magnitude(float a, float b)
 }
 
 constexpr u32 kInfBits = 0x7F800000u;
+constexpr float kInf = __builtin_huge_valf();
 
 /// The power of two that brings a finite magnitude to [128, 256).
 __device__ __forceinline__ float scale_of(u32 largest)
@@ -287,24 +288,33 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                 const float2 y = fma(Two(v[k], v[k + 1]) * b2, one, g2 * g2 * a2).get();
                 m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
             }
-            [[maybe_unused]] float m_most = 0.f, v_most = 0.f;
+            [[maybe_unused]] float m_most = 0.f;
+            float v_most = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-            {
-                // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
-                float floor;
-                asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
-                float rest;
-                const float root = sqrt_fast(floor, rest);
-                // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
-                r[k] = BITS == 8 ? root + rest : root;
-                now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
-                if constexpr (BITS == 8)
+                v_most = max_magnitude(v_most, v[k]);
+            auto update = [&]<bool INFINITE>() {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
                 {
-                    m_most = max_magnitude(m_most, m[k]);
-                    v_most = max_magnitude(v_most, v[k]);
+                    // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
+                    float floor;
+                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
+                    float rest;
+                    float root = sqrt_fast(floor, rest);
+                    // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
+                    r[k] = BITS == 8 ? root + rest : root;
+                    if (INFINITE && v[k] == kInf)  // of a finite gradient whose square is not: no step
+                        root = r[k] = kInf;
+                    now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
+                    if constexpr (BITS == 8)
+                        m_most = max_magnitude(m_most, m[k]);
                 }
-            }
+            };
+            if (v_most < kInf)
+                update.template operator()<false>();
+            else
+                update.template operator()<true>();
             if constexpr (MASTER)
                 store8(master, now);
             if (whole)

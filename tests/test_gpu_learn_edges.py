@@ -107,3 +107,49 @@ def test_adamw_refuses_moments_off_a_vector_boundary(bits):
     assert torch.equal(p, before)
     for k in names:
         assert torch.equal(moved[k].view(torch.uint8), other[k].view(torch.uint8))
+
+
+HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+
+
+def formula(p, g, m, v, step, *, lr, betas, eps, weight_decay):
+    """A step in 64 bits but for g * g and v, which overflow where 32 bits do. Returns the parameter, the moments and the
+    tolerance of the parameter: a rounding of each product, sum, root and quotient of the part that moves, the decay's."""
+    b1, b2 = betas
+    size = m.abs() * b1 + g.abs() * (1 - b1)
+    m, v = m * b1 + g * (1 - b1), v * b2 + (g.float() * g.float()).double() * (1 - b2)
+    den = (v / (1 - b2 ** step)).sqrt() + eps
+    new = p * (1 - lr * weight_decay) - lr * (m / (1 - b1 ** step)) / den
+    return new, m, v, 4 * EPS * p.abs() + 24 * EPS * lr * size / (1 - b1 ** step) / den
+
+
+@pytest.mark.parametrize("dtype,grad_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                              (torch.float16, torch.float32)])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [False, True])
+def test_adamw_takes_no_step_where_the_square_of_a_finite_gradient_is_infinite(dtype, grad_dtype, bits, master):
+    """v is infinite there, m / inf is zero: the parameter decays, and its neighbours go on as ever. With 32-bit moments
+    it stays so; 8 bits have no infinity to hold v by."""
+    params = [randn(n, seed=n).to(dtype) for n in (700, 256, 9)]
+    state = learn.adamw_state(params, bits=bits, master=master)
+    large = torch.zeros(700, dtype=torch.bool, device="cuda")
+    large[[0, 8, 255, 256, 511, 699]] = True
+    m, v = torch.zeros(700, dtype=torch.float64, device="cuda"), torch.zeros(700, dtype=torch.float64, device="cuda")
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for step in (1, 2, 3) if bits == 32 else (1,):
+        grads = [randn(p.numel(), seed=10 * step + i, scale=0.1).to(grad_dtype) for i, p in enumerate(params)]
+        if step == 1:
+            grads[0][large] = torch.tensor([2e19, -2e19, 1e20, 3e38, -3e38, 1e30], device="cuda").to(grad_dtype)
+        p = (state["master"][:700] if master else params[0]).double()
+        learn.adamw_step(params, grads, step=step, **HYPER, **state)
+        new, m, v, tol = formula(p, grads[0].double(), m, v, step, **HYPER)
+        assert v[large].isinf().all() and v[~large].isfinite().all() and m.isfinite().all()
+        assert torch.equal(new[large], (p * (1 - 1e-2 * 0.1))[large])
+        if master:
+            assert ((state["master"][:700].double() - new).abs() <= tol).all()
+        assert ((params[0].double() - new).abs() <= tol + half * new.abs() * 1.01).all()
+        assert all(q.isfinite().all() for q in params)
+    if bits == 32:
+        assert state["exp_avg_sq"][:700][large].isinf().all() and state["exp_avg"].isfinite().all()
+    else:
+        assert state["exp_avg_sq"][:700].float().isnan().equal(large)
