@@ -520,8 +520,8 @@ typedef struct b2_adamw_args {
  * one of the two codes about it, at random by (seed, step, element) with the odds that keep the mean of its square; a
  * positive one of at least 2^-126 keeps at least the smallest code. A parameter with a NaN or infinite gradient becomes
  * NaN or infinite and leaves the others of its block alone. A finite gradient whose square passes the largest 32-bit
- * number (from 1.8e19 on) makes v infinite: the parameter decays and takes no step. It stays so in 32 bits; 8-bit codes
- * have no infinity, v is stored as NaN and the next step spoils the parameter. */
+ * number (from 1.8e19 on) makes v infinite: the parameter decays and takes no step, then and afterwards. 8-bit codes
+ * have no infinity: NaN stands for it in exp_avg_sq. */
 b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -135,12 +135,17 @@ __device__ __forceinline__ float reciprocal_fast(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-/// The larger magnitude; NaN if either is.
-__device__ __forceinline__ float max_magnitude(float a, float b)
+/// The largest magnitude of three or of eight; NaN if one is.
+__device__ __forceinline__ float max_magnitude(float a, float b, float c)
 {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+__device__ __forceinline__ float max_magnitude(const float (&x)[8])
+{
+    const float a = max_magnitude(x[0], x[1], x[2]), b = max_magnitude(x[3], x[4], x[5]);
+    return max_magnitude(max_magnitude(a, x[6], x[7]), b, b);
 }
 
 constexpr u32 kInfBits = 0x7F800000u;
@@ -288,12 +293,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                 const float2 y = fma(Two(v[k], v[k + 1]) * b2, one, g2 * g2 * a2).get();
                 m[k] = x.x, m[k + 1] = x.y, v[k] = y.x, v[k + 1] = y.y;
             }
-            [[maybe_unused]] float m_most = 0.f;
-            float v_most = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v_most = max_magnitude(v_most, v[k]);
-            auto update = [&]<bool INFINITE>() {
+            [[maybe_unused]] float v_most = 0.f;
+            auto update = [&]<bool ODD>() {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                 {
@@ -304,14 +305,19 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                     float root = sqrt_fast(floor, rest);
                     // for a code with what is left of it: a unit in the last place moves a few codes to their neighbours
                     r[k] = BITS == 8 ? root + rest : root;
-                    if (INFINITE && v[k] == kInf)  // of a finite gradient whose square is not: no step
-                        root = r[k] = kInf;
-                    now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
+                    // No step where v is infinite, the square of a finite gradient: its root above is NaN. 8-bit codes have no
+                    // infinity, NaN stands for it; the minimum takes the number of the two (the first moment holds a
+                    // NaN of the gradient's own).
                     if constexpr (BITS == 8)
-                        m_most = max_magnitude(m_most, m[k]);
+                        asm("min.f32 %0, %0, %1;" : "+f"(root) : "f"(kInf));
+                    else if (ODD && v[k] == kInf)
+                        root = kInf;
+                    now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
+                    if (BITS == 8 && k & 1)
+                        v_most = max_magnitude(v_most, v[k - 1], v[k]);
                 }
             };
-            if (v_most < kInf)
+            if (BITS == 8 || max_magnitude(v) < kInf)
                 update.template operator()<false>();
             else
                 update.template operator()<true>();
@@ -333,7 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
             }
             else
             {
-                u32 top = largest_of(m_most, m);
+                u32 top = largest_of(max_magnitude(m), m);
                 bool bad = top >> 31;
                 const float ms = scale_of(top), mi = inverse_power(ms);
 #pragma unroll

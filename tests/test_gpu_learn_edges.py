@@ -153,3 +153,22 @@ def test_adamw_takes_no_step_where_the_square_of_a_finite_gradient_is_infinite(d
         assert state["exp_avg_sq"][:700][large].isinf().all() and state["exp_avg"].isfinite().all()
     else:
         assert state["exp_avg_sq"][:700].float().isnan().equal(large)
+
+
+@pytest.mark.parametrize("master", [False, True])
+def test_adamw_8_bit_codes_hold_an_infinite_second_moment_as_nan(master):
+    """It stays infinite: the parameter decays and takes no step, on later steps too. A gradient's own NaN is held by the
+    first moment and goes on spoiling its parameter."""
+    p = randn(512, seed=1)
+    state = learn.adamw_state([p], bits=8, master=master)
+    want = p.clone()
+    for step in range(1, 5):
+        g = randn(512, seed=10 + step)
+        if step == 1:
+            g[7], g[300], g[9] = 2e19, -3e38, float("nan")
+        learn.adamw_step([p], [g], step=step, **HYPER, **state)
+        want = want * (1 - 1e-2 * 0.1)
+        assert p[9].isnan() and torch.cat((p[:9], p[10:])).isfinite().all()
+        # two roundings each step (of the factor, of the product), on both sides
+        assert all(abs(float(p[i] - want[i])) <= 4 * step * EPS * abs(float(want[i])) for i in (7, 300))
+    assert state["exp_avg_sq"].float().isnan().nonzero().flatten().tolist() == [7, 9, 300]
