@@ -518,10 +518,12 @@ typedef struct b2_adamw_args {
  * with m' = m / (1 - beta1^step), v' = v / (1 - beta2^step), in 32 bits, for every tensor: one launch for each 1,000 of
  * them. 8-bit moments are rounded when they are stored: the first to the nearest code, the second (its square root) to
  * one of the two codes about it, at random by (seed, step, element) with the odds that keep the mean of its square; a
- * positive one of at least 2^-126 keeps at least the smallest code. A parameter with a NaN or infinite gradient becomes
- * NaN or infinite and leaves the others of its block alone. A finite gradient whose square passes the largest 32-bit
- * number (from 1.8e19 on) makes v infinite: the parameter decays and takes no step, then and afterwards. 8-bit codes
- * have no infinity: NaN stands for it in exp_avg_sq. */
+ * positive one above 2^-126 keeps at least the smallest code, unless the block's largest is below 2^-124: such blocks are
+ * held as zero. Where v is zero its root is taken as 2^-63 (with eps = 0 nothing is divided by zero), with 8-bit moments
+ * wherever v is below 2^-126.
+ * A parameter with a NaN or infinite gradient becomes NaN or infinite and leaves the others of its block alone. A finite
+ * gradient whose square passes the largest 32-bit number (from 1.8e19 on) makes v infinite: the parameter decays and
+ * takes no step, then and afterwards. 8-bit codes have no infinity: NaN stands for it in exp_avg_sq. */
 b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -16,6 +16,7 @@ constexpr u32 kWarps = 8;
 struct Hyper
 {
     float b1, a1, b2, a2, decay, correct, eps, rate;
+    bool small_eps;  // beside it a root of 2^-63 counts
     float one;  // 1: a sum of two products written as a fused multiplication by it is not fused with either of them
 };
 
@@ -151,11 +152,13 @@ __device__ __forceinline__ float max_magnitude(const float (&x)[8])
 constexpr u32 kInfBits = 0x7F800000u;
 constexpr float kInf = __builtin_huge_valf();
 
-/// The power of two that brings a finite magnitude to [128, 256).
+/// The power of two that brings a finite magnitude to [128, 256); the least one (2^-126) for magnitudes with an exponent
+/// below `LEAST` (as in their bits), which then count as zero.
+template<u32 LEAST>
 __device__ __forceinline__ float scale_of(u32 largest)
 {
     const u32 e = largest & kInfBits;
-    return __uint_as_float(e > (8u << 23) ? e - (7u << 23) : 1u << 23);
+    return __uint_as_float(e >= (LEAST << 23) ? e - (7u << 23) : 1u << 23);
 }
 /// 1 / scale, exactly.
 __device__ __forceinline__ float inverse_power(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                 {
-                    // normal numbers, and no division by zero: a second moment below 2^-126 counts as zero
+                    // normal numbers, and no division by zero
                     float floor;
                     asm("max.NaN.f32 %0, %1, %2;" : "=f"(floor) : "f"(v[k]), "f"(0x1p-126f));
                     float rest;
@@ -310,14 +313,14 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                     // NaN of the gradient's own).
                     if constexpr (BITS == 8)
                         asm("min.f32 %0, %0, %1;" : "+f"(root) : "f"(kInf));
-                    else if (ODD && v[k] == kInf)
-                        root = kInf;
+                    else if (ODD)
+                        root = v[k] == kInf ? kInf : v[k] > 0.f && v[k] < 0x1p-126f ? __fsqrt_rn(v[k]) : root;
                     now[k] = now[k] * h.decay - m[k] * (h.rate * reciprocal_fast(root * h.correct + h.eps));
                     if (BITS == 8 && k & 1)
                         v_most = max_magnitude(v_most, v[k - 1], v[k]);
                 }
             };
-            if (BITS == 8 || max_magnitude(v) < kInf)
+            if (BITS == 8 || (!h.small_eps && max_magnitude(v) < kInf))
                 update.template operator()<false>();
             else
                 update.template operator()<true>();
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
             {
                 u32 top = largest_of(max_magnitude(m), m);
                 bool bad = top >> 31;
-                const float ms = scale_of(top), mi = inverse_power(ms);
+                const float ms = scale_of<9>(top), mi = inverse_power(ms);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     m[k] *= mi;
@@ -354,7 +357,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                 top = __reduce_max_sync(~0u, __float_as_uint(v_most));
                 bad = top >= kInfBits;
                 top = bad ? largest_of(__uint_as_float(top), r) : __float_as_uint(__fsqrt_rn(__uint_as_float(top)));
-                const float vs = scale_of(top);
+                // Roots of less than 2^-62 are held as zero (zeros come as 2^-63): under the least scale the factors below
+                // wrap around to less than 2^-100, the smallest code stands for 2^-135 and its square is zero.
+                const float vs = scale_of<65>(top);
                 const u32 vs_exponent = __float_as_uint(vs) - (127u << 23);
                 const u32 pair = block * (kMoment / 2) + i0 / 2;  // of the element among all, modulo 2^32
                 float code[8];
@@ -431,7 +436,8 @@ void run(const b2_ctx& ctx, const b2_adamw_args& a, cudaStream_t st)
     const double c2 = 1 - std::pow(a.beta2, static_cast<double>(a.step));
     const Hyper h{static_cast<float>(a.beta1), static_cast<float>(1 - a.beta1), static_cast<float>(a.beta2),
                   static_cast<float>(1 - a.beta2), static_cast<float>(1 - a.lr * a.weight_decay),
-                  static_cast<float>(1 / std::sqrt(c2)), static_cast<float>(a.eps), static_cast<float>(a.lr / c1), 1.f};
+                  static_cast<float>(1 / std::sqrt(c2)), static_cast<float>(a.eps), static_cast<float>(a.lr / c1),
+                  a.eps < 0x1p-38 / std::sqrt(c2), 1.f};
     constexpr u32 kFew = 96, kMany = 1000;
     for (u32 first = 0; first < a.count;)
     {

@@ -172,3 +172,44 @@ def test_adamw_8_bit_codes_hold_an_infinite_second_moment_as_nan(master):
         # two roundings each step (of the factor, of the product), on both sides
         assert all(abs(float(p[i] - want[i])) <= 4 * step * EPS * abs(float(want[i])) for i in (7, 300))
     assert state["exp_avg_sq"].float().isnan().nonzero().flatten().tolist() == [7, 9, 300]
+
+
+@pytest.mark.parametrize("master", [False, True])
+def test_adamw_without_eps_takes_second_moments_below_the_normal_numbers_as_they_are(master):
+    """32-bit moments. v is subnormal, of 2^-149 steps: three roundings of it come to the tolerance. Where the gradient is
+    zero nothing moves."""
+    hyper = dict(lr=1e-2, betas=(0.9, 0.9), eps=0.0, weight_decay=0.0)
+    u = torch.rand(600, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    g = (u + 1) * 1e-19 * torch.where(u * 16 % 1 < 0.5, -1.0, 1.0)
+    g[::7] = 0.0
+    g[5::50] = 1.0  # normal numbers beside them
+    p = randn(600, seed=2)
+    state, before = learn.adamw_state([p], master=master), p.double()
+    learn.adamw_step([p], [g], step=1, master=state.pop("master", None), **hyper, **state)
+    zero = torch.zeros(600, dtype=torch.float64, device="cuda")
+    live = g != 0
+    new, _, _, tol = formula(before, g.double(), zero, zero, 1, **hyper)
+    v = 0.1 * g.double() ** 2
+    tol = tol + hyper["lr"] * 3 * 2.0 ** -149 / v
+    assert float(v[live].min()) < 2.0 ** -126 and float(v[live].min()) > 2.0 ** -140
+    assert ((p.double() - new).abs() <= tol)[live].all()
+    assert torch.equal(p[~live].double(), before[~live])
+
+
+def test_adamw_8_bits_hold_second_moments_below_the_normal_numbers_as_zero():
+    """Zeros among them stay zero, as they do beside an infinity or a NaN."""
+    n = 256 * 5
+    g = torch.zeros(n, device="cuda")
+    g[:256:2] = 1e-20                       # a block of them and of zeros
+    g[256:512] = 1e-25                      # of them alone
+    g[512], g[768], g[769] = INF, 2e19, 1e-20  # zeros beside infinities
+    g[1024:1030] = 1.0
+    g[1100] = 1e-20                         # one beside normal numbers
+    p = randn(n, seed=1)
+    state = learn.adamw_state([p], bits=8)
+    learn.adamw_step([p], [g], step=1, **HYPER, **state)
+    code = state["exp_avg_sq"].float()
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[[512, 768]] = True
+    assert code[bad].isnan().all() and (code[1024:1030] > 0).all()
+    assert (torch.cat((code[:1024][~bad[:1024]], code[1030:])) == 0).all()
