@@ -418,6 +418,8 @@ void launch(const b2_ctx& ctx, const b2_adamw_args& a, u32 first, u32 count, con
         t.e[i] = {x.param, x.grad, x.elements, x.block, static_cast<u32>(blocks)};
         blocks += (x.elements + kMoment - 1) / kMoment;
     }
+    if (!blocks)  // empty tensors alone
+        return;
     t.blocks = static_cast<u32>(blocks);
     const u32 key = mix(mix(a.seed) ^ static_cast<u32>(a.step));
     const Moments s{a.exp_avg, a.exp_avg_sq, a.exp_avg_scale, a.exp_avg_sq_scale, a.master};

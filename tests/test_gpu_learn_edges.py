@@ -213,3 +213,23 @@ def test_adamw_8_bits_hold_second_moments_below_the_normal_numbers_as_zero():
     bad[[512, 768]] = True
     assert code[bad].isnan().all() and (code[1024:1030] > 0).all()
     assert (torch.cat((code[:1024][~bad[:1024]], code[1030:])) == 0).all()
+
+
+def test_adamw_takes_any_number_of_empty_tensors():
+    """Through the C ABI: a launch's worth of them (1,000) before, after and between tensors with elements."""
+    L, h = _lib.lib(), default_context().handle
+    for places in ([1000], [0], [999], [3, 2500]):
+        params = [randn(300, seed=i) for i in range(len(places))]
+        want = [p.clone() for p in params]
+        g = randn(300, seed=9)
+        state = learn.adamw_state(params)
+        table = (_lib.AdamwTensor * 3001)()
+        for i, (place, p) in enumerate(zip(places, params)):
+            table[place] = _lib.AdamwTensor(p.data_ptr(), g.data_ptr(), 300, 2 * i, 0)
+        a = _lib.AdamwArgs()
+        a.tensors, a.count, a.moment_bits, a.blocks = C.addressof(table), 3001, 32, 2 * len(places)
+        a.exp_avg, a.exp_avg_sq = state["exp_avg"].data_ptr(), state["exp_avg_sq"].data_ptr()
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay, a.step = 1e-3, 0.9, 0.999, 1e-8, 1e-2, 1
+        assert L.b2_adamw(h, C.byref(a), None) == 0, _lib.last_error()
+        learn.adamw_step(want, [g] * len(places), step=1, **learn.adamw_state(want))
+        assert all(torch.equal(p, q) for p, q in zip(params, want))
