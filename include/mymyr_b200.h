@@ -417,8 +417,8 @@ void b2_env_destroy(b2_env* env);
 /* ------------------------------------------------------------------------------------------------ learner
  * Operators of a policy trained over the environments and expansions above: embedding lookup, log-probabilities of
  * given tokens (actions) and the AdamW step. They have no counterpart in the reference. Every call is asynchronous on
- * `stream`, allocates nothing and can be captured in a CUDA graph; device memory is the caller's. Calls on a context
- * run on its device and leave the thread's current device as it was. */
+ * `stream` and allocates nothing; device memory is the caller's. Calls on a context run on its device and leave the
+ * thread's current device as it was. All but b2_adamw can be captured in a CUDA graph. */
 enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };
 
 enum { B2_TOP_MAX = 32 };
@@ -523,7 +523,9 @@ typedef struct b2_adamw_args {
  * wherever v is below 2^-126.
  * A parameter with a NaN or infinite gradient becomes NaN or infinite and leaves the others of its block alone. A finite
  * gradient whose square passes the largest 32-bit number (from 1.8e19 on) makes v infinite: the parameter decays and
- * takes no step, then and afterwards. 8-bit codes have no infinity: NaN stands for it in exp_avg_sq. */
+ * takes no step, then and afterwards. 8-bit codes have no infinity: NaN stands for it in exp_avg_sq.
+ * A captured call would repeat one step's corrections and random numbers on every replay: B2_UNSUPPORTED on a stream
+ * under capture. */
 b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -501,6 +501,12 @@ extern "C" b2_status b2_adamw(b2_ctx* ctx, const b2_adamw_args* args, void* stre
             throw bad("moments and master must start on a boundary of eight elements (32 bytes, 8 for 8-bit moments)");
         const OnDevice on(ctx->device);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        // the corrections and the rounding's random numbers are those of `step`, which a graph would hold for good
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(st, &capture) != cudaSuccess)
+            cudaGetLastError();  // the launch will say
+        if (capture != cudaStreamCaptureStatusNone)
+            throw Error(B2_UNSUPPORTED, "b2_adamw: a step is of its own number and cannot be captured in a graph");
         dispatch_dtype(a.param_dtype, "b2_adamw", [&]<class P>() {
             if (a.grad_dtype == a.param_dtype)
                 run<P, P>(*ctx, a, st);

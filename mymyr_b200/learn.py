@@ -4,7 +4,8 @@ actions, with entropy and the best alternatives, and their gradient) and the Ada
 at once (``AdamW``, ``adamw_step``). The first two take part in torch's autograd.
 
 Work runs on the tensors' device, on torch's current stream there or on the raw stream handle ``stream``, and is
-asynchronous. Statistics and sums are 32-bit whatever the tensors' type (float32, bfloat16 or float16)."""
+asynchronous. All but the AdamW step can be captured in CUDA graphs. Statistics and sums are 32-bit whatever the
+tensors' type (float32, bfloat16 or float16)."""
 
 from __future__ import annotations
 
@@ -141,7 +142,9 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
     A gradient is of its parameter's type or float32; one that is None leaves its tensor alone. Parameters of 16 bits
     are rounded to nearest from ``master`` if given. 8-bit moments are rounded for storage only: the first to nearest,
     the second to one of its two neighbours by random numbers of (``seed``, step, element), so that the small steps of
-    a slow average are kept in the mean."""
+    a slow average are kept in the mean.
+
+    A CUDA graph would repeat one step's corrections and random numbers: a call on a stream under capture is refused."""
     params, grads = list(params), list(grads)
     with contextlib.nullcontext() if stream is None else _on(stream, exp_avg, exp_avg_sq, exp_avg_scale,
                                                             exp_avg_sq_scale, master, *params, *grads):

@@ -233,3 +233,28 @@ def test_adamw_takes_any_number_of_empty_tensors():
         assert L.b2_adamw(h, C.byref(a), None) == 0, _lib.last_error()
         learn.adamw_step(want, [g] * len(places), step=1, **learn.adamw_state(want))
         assert all(torch.equal(p, q) for p, q in zip(params, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_a_graph(bits):
+    """Its replays would repeat one step's corrections, and with 8 bits its random numbers. Nothing is launched; the step
+    outside of the capture is taken as ever, and a graph of the other operators stands."""
+    p, g = randn(700, seed=1).requires_grad_(True), randn(700, seed=2)
+    before = p.detach().clone()
+    state = learn.adamw_state([p], bits=bits)
+    opt = learn.AdamW([p], bits=bits)
+    p.grad = g
+    x = randn(5, 40, seed=3)
+    want = learn.logprobs(x).entropy
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = learn.logprobs(x).entropy
+        with pytest.raises(ValueError, match="captured"):
+            learn.adamw_step([p], [g], step=1, **state)
+        with pytest.raises(ValueError, match="captured"):
+            opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(p.detach(), before)
+    learn.adamw_step([p], [g], step=1, **state)
+    assert not torch.equal(p.detach(), before)
