@@ -155,7 +155,9 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
 class AdamW:
     """AdamW over a policy's parameters, all of a group's tensors in one launch (``adamw_step``). ``params``: tensors,
     or groups as dicts with "params" and their own lr, betas, eps or weight_decay. ``bits``: 32 or 8 for the moments;
-    ``master``: 32-bit copies of 16-bit parameters. Each group keeps its moments in flat tensors of its own."""
+    ``master``: 32-bit copies of 16-bit parameters. Each group keeps its moments in flat tensors of its own. A parameter's
+    step number, by which its averages are corrected, counts the steps that it had a gradient for; where a group's differ
+    (some had none at times), each number is a launch."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, bits: int = 32, master: bool = False, seed: int = 0):
@@ -164,6 +166,7 @@ class AdamW:
         groups = params if params and isinstance(params[0], dict) else [{"params": params}]
         self.param_groups = [defaults | g | {"params": list(g["params"])} for g in groups]
         self.steps = 0
+        self.param_steps = [[0] * len(g["params"]) for g in self.param_groups]
         self.seed = int(seed)
         self.state = [adamw_state(g["params"], bits=bits, master=master) for g in self.param_groups]
 
@@ -175,15 +178,21 @@ class AdamW:
 
     def step(self, stream=None) -> None:
         """Updates every parameter that has a gradient."""
-        self.steps += 1
         with torch.no_grad():
-            for i, (g, s) in enumerate(zip(self.param_groups, self.state)):
-                adamw_step(g["params"], [p.grad for p in g["params"]], step=self.steps, lr=g["lr"], betas=g["betas"],
-                           eps=g["eps"], weight_decay=g["weight_decay"], seed=self.seed + i, stream=stream, **s)
+            for i, (g, s, counts) in enumerate(zip(self.param_groups, self.state, self.param_steps)):
+                grads = [p.grad for p in g["params"]]
+                now = [n if x is None else n + 1 for n, x in zip(counts, grads)]
+                for step in sorted({n for n, x in zip(now, grads) if x is not None}):
+                    adamw_step(g["params"], [x if n == step else None for n, x in zip(now, grads)], step=step, lr=g["lr"],
+                               betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], seed=self.seed + i,
+                               stream=stream, **s)
+                counts[:] = now
+        self.steps += 1
 
     def state_dict(self) -> dict:
-        """The step count, the groups' options and their moments (the tensors themselves, not copies)."""
-        return {"steps": self.steps, "seed": self.seed, "state": self.state,
+        """The step counts, the groups' options and their moments (the tensors themselves, not copies)."""
+        return {"steps": self.steps, "param_steps": [list(c) for c in self.param_steps], "seed": self.seed,
+                "state": self.state,
                 "groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
 
     def load_state_dict(self, state: dict) -> None:
@@ -194,9 +203,14 @@ class AdamW:
             if mine.keys() != given.keys() or any(mine[k].shape != given[k].shape or mine[k].dtype != given[k].dtype
                                                   for k in mine):
                 raise ValueError("AdamW: moments of other sizes or types")
+        # without counts of their own (of an earlier version) all parameters are at the optimizer's step
+        counts = state.get("param_steps") or [[int(state["steps"])] * len(c) for c in self.param_steps]
+        if [len(c) for c in counts] != [len(c) for c in self.param_steps]:
+            raise ValueError("AdamW: another number of parameters")
         for mine, given in zip(self.state, state["state"]):
             for k in mine:
                 mine[k].copy_(given[k])
         for g, options in zip(self.param_groups, state["groups"]):
             g.update(options)
         self.steps, self.seed = int(state["steps"]), int(state["seed"])
+        self.param_steps = [[int(n) for n in c] for c in counts]

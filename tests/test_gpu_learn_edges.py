@@ -258,3 +258,66 @@ def test_adamw_refuses_a_graph(bits):
     assert torch.equal(got, want) and torch.equal(p.detach(), before)
     learn.adamw_step([p], [g], step=1, **state)
     assert not torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_corrects_each_parameter_by_its_own_steps(bits):
+    """A parameter whose first gradient comes late moves by the learning rate on its first step, whatever the others'
+    count; with weights of one sign of gradient only, m' / sqrt(v') is 1 up to the roundings (8-bit codes: half of 2^-4 of
+    the first moment, one of 2^-3 of the second's root, none of which has come in on a first step)."""
+    a, b = (torch.zeros(300, device="cuda", requires_grad=True) for _ in range(2))
+    opt = learn.AdamW([a, b], lr=1e-2, weight_decay=0.0, bits=bits)
+    for step in range(1, 12):
+        a.grad = torch.ones_like(a)
+        b.grad = torch.full_like(b, -3.0) if step == 11 else None
+        opt.step()
+    assert float((b.detach() - 1e-2).abs().max()) <= 32 * EPS * 1e-2 + 1e-2 * 1e-8 / 3
+    assert opt.steps == 11 and opt.param_steps == [[11, 1]]
+
+
+def test_adamw_object_with_gradients_now_and_then():
+    """As torch's, which counts each parameter's steps; and its state, with and without counts of its own."""
+    shapes = [(30, 20), (20,), (300,), (7,)]
+
+    def make():
+        params = [randn(*s, seed=i).requires_grad_(True) for i, s in enumerate(shapes)]
+        return params, [{"params": params[:3]}, {"params": params[3:], "lr": 3e-3}]
+
+    def give(params, step):
+        for i, p in enumerate(params):
+            p.grad = None if (step + i) % (i + 1) else randn(*p.shape, seed=100 * step + i)
+
+    mine, groups = make()
+    opt = learn.AdamW(groups, lr=1e-2, weight_decay=0.1)
+    other, groups = make()
+    ref = torch.optim.AdamW(groups, lr=1e-2, weight_decay=0.1)
+    steps = 13
+    saved = None
+    for step in range(1, steps + 1):
+        for params, o in ((mine, opt), (other, ref)):
+            give(params, step)
+            o.step()
+        if step == 6:
+            saved = opt.state_dict()
+            saved["state"] = [{k: t.clone() for k, t in s.items()} for s in saved["state"]]
+            at = [p.detach().clone() for p in mine]
+    for p, q in zip(mine, other):
+        # on both sides a step rounds the parameter four times and its part of up to 10 learning rates 24 times
+        tol = 2 * steps * EPS * (4 * float(q.detach().abs().max()) + 24 * 10 * 1e-2)
+        assert float((p - q).detach().abs().max()) <= tol
+    assert opt.param_steps == [[13, 7, 5], [4]]
+    again, groups = make()
+    with torch.no_grad():
+        for p, x in zip(again, at):
+            p.copy_(x)
+    late = learn.AdamW(groups, lr=1e-2, weight_decay=0.1)
+    late.load_state_dict(saved)
+    for step in range(7, steps + 1):
+        give(again, step)
+        late.step()
+    assert all(torch.equal(p, q) for p, q in zip(mine, again)) and late.param_steps == opt.param_steps
+    old = {k: v for k, v in saved.items() if k != "param_steps"}
+    late.load_state_dict(old)
+    assert late.steps == 6 and late.param_steps == [[6, 6, 6], [6]]
+    with pytest.raises(ValueError):
+        late.load_state_dict(saved | {"param_steps": [[1, 2], [3]]})
