@@ -149,9 +149,10 @@ struct Row
     __device__ __forceinline__ Row(const Sums& a, float inv_temperature)
         : ref(a.ref), inv_t(inv_temperature), dead(a.best == -kInf && a.s == a.s), bad(a.s != a.s)
     {
-        log2_s = __log2f(a.s);
+        // in full, once for a row: the results of a nearly sure row are small beside the error of the fast forms
+        log2_s = log2f(a.s);
         log_s = dead ? -kInf : log2_s * kLn2;
-        entropy = dead ? 0.f : (log2_s - __fdividef(a.t, a.s)) * kLn2;
+        entropy = dead ? 0.f : (log2_s - a.t / a.s) * kLn2;
     }
     __device__ __forceinline__ float logp(float x) const
     {

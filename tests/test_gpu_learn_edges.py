@@ -61,6 +61,33 @@ def test_statistics_off_a_16_byte_boundary_are_refused():
     assert (out > 0).all()
 
 
+def check_sure_rows(width, rows, least, most):
+    """A row of one logit of 0, one of -x and no others that count, in any order: S = 1 + exp(-x). Its one rounding is at
+    most EPS, and passes to the log-probability (-log S) and the entropy as it is. exp(-x) itself is off by 4 EPS of its
+    value and by the roundings of its exponent, 2 EPS of x each, then the product with x, and the quotient and log by a
+    unit or two of their own small value."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    i = torch.arange(rows, device="cuda")
+    x = torch.full((rows, width), -200.0, device="cuda")
+    a = torch.randint(0, width, (rows,), generator=g, device="cuda")
+    b = (a + 1 + torch.randint(0, width - 1, (rows,), generator=g, device="cuda")) % width
+    x[i, b] = -(least + (most - least) * torch.rand(rows, generator=g, device="cuda"))
+    x[i, a] = 0.0
+    got = learn.logprobs(x, a, top=1)
+    d = -x[i, b].double()
+    e = (-d).exp()
+    logp = -torch.log1p(e)
+    entropy = -logp + e * d / (1 + e)
+    assert ((got.logprob.double() - logp).abs() <= EPS * (1 + e * (4 * d + 12))).all()
+    assert ((got.entropy.double() - entropy).abs() <= EPS * (1 + e * (d + 1) * (4 * d + 12))).all()
+    assert torch.equal(got.top_tokens[:, 0], a)
+
+
+@pytest.mark.parametrize("width", [2, 20, 40, 128])
+def test_logprobs_of_sure_rows_are_right_to_a_rounding_of_their_sum(width):
+    check_sure_rows(width, 5000, 7.0, 16.0)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("first", [0, 17])
 def test_gradient_of_a_vector_without_rows(dtype, first):
