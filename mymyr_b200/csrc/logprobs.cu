@@ -25,7 +25,11 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr float kAhead = 60.f;  // a sum's reference follows the row's maximum when it is this far ahead, in powers of two
+/// A thread's reference follows its largest logit when that is this far ahead, in powers of two. Moving it by L cancels in
+/// t what L times s had added, so a long way costs digits (rows of 70,001 normal logits of deviation 8: entropy off by 59
+/// units of 2^-24 with 60, 8 with 10, 8 with 0), a short one time (8,192 rows of 65,536 bf16: 181 us with 60 and with 10,
+/// 193 with 2, 205 with 0).
+constexpr float kAhead = 10.f;
 
 /// The rows of a call: row r's logits and mask, and its length, always inside the arrays.
 struct Rows

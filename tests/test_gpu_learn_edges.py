@@ -88,6 +88,28 @@ def test_logprobs_of_sure_rows_are_right_to_a_rounding_of_their_sum(width):
     check_sure_rows(width, 5000, 7.0, 16.0)
 
 
+@pytest.mark.parametrize("width,rows", [(200, 5000), (3000, 2000), (70001, 300), (300000, 3)])
+def test_logprobs_of_long_sure_rows_are_right_to_a_rounding_of_their_sum(width, rows):
+    """Wherever the largest logit stands. It is more than 2^10 (6.94 as a logarithm) ahead of all others, so a thread's
+    running reference moves to it, and its own term is exactly one."""
+    check_sure_rows(width, rows, 7.0, 41.0)
+
+
+@pytest.mark.parametrize("width,rows", [(3000, 600), (70001, 100)])
+def test_entropy_of_spread_rows(width, rows):
+    """Normal logits of deviation 8: a few count. A thread's reference lags behind by at most 2^10, so t holds up to ten
+    times s more than it is to: three roundings of that when it moves, 6.93 * 3 EPS; two exponentials of 4 EPS; the
+    roundings of exponents (2 EPS of d each, d weighted by its share: below the entropy and one) and of the sums (few
+    terms count: six roundings of positive ones)."""
+    x = randn(rows, width, seed=width, scale=8.0)
+    lp = torch.log_softmax(x.double(), 1)
+    want = torch.special.entr(lp.exp()).sum(1)
+    h = float(want.max())
+    got = learn.logprobs(x).entropy.double()
+    assert h < 4
+    assert float((got - want).abs().max()) <= EPS * (6.93 * 3 + 8 + 2 * (h + 1) + 6)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("first", [0, 17])
 def test_gradient_of_a_vector_without_rows(dtype, first):
