@@ -89,6 +89,22 @@ int32_t index_bits(const Tensor& t, const Tensor& with, const char* message)
     return t.scalar_type() == at::kLong ? 64 : 32;
 }
 
+at::ScalarType float_type(int32_t dtype)
+{
+    return dtype == B2_F32 ? at::kFloat : dtype == B2_BF16 ? at::kBFloat16 : at::kHalf;
+}
+
+at::ScalarType index_type(int32_t bits) { return bits == 64 ? at::kLong : at::kInt; }
+
+/// A tensor that the backward pass finds saved, if it is of the type, the sizes and on the device that it had: hooks on
+/// saved tensors hand back what they will.
+const Tensor& as_saved(const Tensor& t, at::ScalarType type, at::IntArrayRef sizes, at::Device device)
+{
+    refuse(!t.defined() || t.scalar_type() != type || t.device() != device || t.sizes() != sizes,
+           "a saved tensor came back with another type, size or device");
+    return t;
+}
+
 /// Rows with unit column stride.
 Tensor unit_columns(const Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
 
@@ -147,6 +163,7 @@ struct LogProbsNode : ag::Function<LogProbsNode>
         node->save_for_backward({logits, call->tokens, call->offsets, call->mask, call->stats});
         node->saved_data["args"] = std::string(reinterpret_cast<const char*>(&call->a), sizeof(call->a));
         node->saved_data["ctx"] = reinterpret_cast<int64_t>(call->ctx);
+        node->saved_data["device"] = static_cast<int64_t>(logits.get_device());
         node->set_materialize_grads(false);
         ag::variable_list out{call->entropy};
         if (call->logprob.defined())
@@ -163,19 +180,37 @@ struct LogProbsNode : ag::Function<LogProbsNode>
     static ag::variable_list backward(ag::AutogradContext* node, ag::variable_list grads)
     {
         const auto saved = node->get_saved_variables();  // throws where one was changed in place since
-        const Tensor& logits = saved[0];
         b2_logprobs_args a;
         std::memcpy(&a, node->saved_data["args"].toStringRef().data(), sizeof(a));
-        // saved tensors may have moved (hooks that pack them)
+        // hooks may have moved them and laid them out anew
+        const auto rows = static_cast<int64_t>(a.rows), width = static_cast<int64_t>(a.width);
+        const bool ragged = a.offsets;
+        const at::Device device(at::kCUDA, static_cast<c10::DeviceIndex>(node->saved_data["device"].toInt()));
+        const std::vector<int64_t> shape = ragged ? std::vector<int64_t>{width} : std::vector<int64_t>{rows, width};
+        const Tensor logits = unit_columns(as_saved(saved[0], float_type(a.dtype), shape, device));
+        const Tensor stats = as_saved(saved[4], at::kFloat, {rows, 4}, device).contiguous();
         a.logits = logits.data_ptr();
-        a.row_stride = saved[2].defined() ? 0 : static_cast<uint64_t>(logits.stride(0));
-        a.tokens = saved[1].defined() ? saved[1].data_ptr() : nullptr;
-        a.offsets = saved[2].defined() ? saved[2].data_ptr() : nullptr;
-        a.mask = saved[3].defined() ? static_cast<const uint8_t*>(saved[3].data_ptr()) : nullptr;
-        a.mask_stride = saved[3].defined() && !saved[2].defined() ? static_cast<uint64_t>(saved[3].stride(0)) : 0;
-        a.stats = saved[4].data_ptr<float>();
+        a.row_stride = ragged ? 0 : static_cast<uint64_t>(logits.stride(0));
+        a.stats = stats.data_ptr<float>();
+        Tensor tokens, offsets, mask;
+        if (a.tokens)
+        {
+            tokens = as_saved(saved[1], index_type(a.token_bits), {rows}, device).contiguous();
+            a.tokens = tokens.data_ptr();
+        }
+        if (ragged)
+        {
+            offsets = as_saved(saved[2], index_type(a.offsets_bits), {rows + 1}, device).contiguous();
+            a.offsets = offsets.data_ptr();
+        }
+        if (a.mask)
+        {
+            mask = unit_columns(as_saved(saved[3], at::kBool, shape, device));
+            a.mask = static_cast<const uint8_t*>(mask.data_ptr());
+            a.mask_stride = ragged ? 0 : static_cast<uint64_t>(mask.stride(0));
+        }
         const Tensor entropy = grads[0].defined() ? grads[0].contiguous() : Tensor();
-        const Tensor logprob = saved[1].defined() && grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor logprob = a.tokens && grads[1].defined() ? grads[1].contiguous() : Tensor();
         Tensor grad;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
@@ -233,6 +268,8 @@ std::array<OptTensor, 4> logprobs(Tensor logits, OptTensor tokens, OptTensor off
         a.token_bits = index_bits(*tokens, logits, "logprobs: tokens must be int32 or int64, on the logits' device");
         refuse(tokens->sizes() != at::IntArrayRef(shape), "logprobs: tokens must have the rows' shape");
         call.tokens = tokens->contiguous();
+        if (call.tokens.dim() != 1)
+            call.tokens = call.tokens.view({static_cast<int64_t>(a.rows)});
         a.tokens = call.tokens.data_ptr();
     }
     if (mask)
@@ -318,8 +355,11 @@ struct EmbeddingNode : ag::Function<EmbeddingNode>
         const auto saved = node->get_saved_variables();
         b2_embedding_args a;
         std::memcpy(&a, node->saved_data["args"].toStringRef().data(), sizeof(a));
-        a.tokens = saved[0].data_ptr();  // it may have moved (hooks that pack it)
         const Tensor grad = unit_columns(grads[0]);
+        // hooks may have moved them and laid them out anew
+        const Tensor tokens =
+            as_saved(saved[0], index_type(a.token_bits), {static_cast<int64_t>(a.count)}, grad.device()).contiguous();
+        a.tokens = tokens.data_ptr();
         Tensor out;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
@@ -343,7 +383,7 @@ Tensor embedding(Tensor tokens, Tensor weight, double scale)
     b2_ctx* const ctx = context(weight.get_device());
     const py::gil_scoped_release unlocked;
     const c10::cuda::CUDAGuard guard(weight.device());
-    const Tensor flat = tokens.contiguous();
+    const Tensor flat = tokens.dim() == 1 ? tokens.contiguous() : tokens.contiguous().view({tokens.numel()});
     weight = unit_columns(weight);
     a.tokens = flat.data_ptr();
     a.dtype = dtype_of(weight, "");

@@ -370,3 +370,68 @@ def test_adamw_object_with_gradients_now_and_then():
     assert late.steps == 6 and late.param_steps == [[6, 6, 6], [6]]
     with pytest.raises(ValueError):
         late.load_state_dict(saved | {"param_steps": [[1, 2], [3]]})
+
+
+# ------------------------------------------------------------------------------------------------ saved tensors
+
+def gradients(x, y, mask, ragged, table, tokens):
+    x, table = x.clone().requires_grad_(True), table.clone().requires_grad_(True)
+    offsets = torch.tensor([0, 40, 40, 160, 201], device="cuda") if ragged else None
+    got = learn.logprobs(x.view(-1) if ragged else x, y[:4] if ragged else y, offsets=offsets,
+                         mask=mask.view(-1) if ragged else mask)
+    rows = learn.embedding(tokens, table, scale=2.0)
+    n = got.entropy.shape[0]
+
+    def actions():
+        return torch.autograd.grad((got.logprob, got.entropy), x, (randn(n, seed=5), randn(n, seed=6)))[0]
+
+    def embeddings():
+        return torch.autograd.grad(rows, table, randn(*rows.shape, seed=7))[0]
+
+    return actions, embeddings
+
+
+def saved_cases():
+    x, y = randn(67, 3, seed=1), torch.randint(0, 3, (67,), generator=torch.Generator(device="cuda").manual_seed(2),
+                                               device="cuda")
+    mask = randn(67, 3, seed=3) > -0.8
+    return x, y, mask, randn(9, 6, seed=4), (y.repeat(2) * 3 % 9).view(2, 67)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_saved_tensors_may_come_back_in_another_layout(ragged):
+    """Hooks that keep them in another order of memory, two elements apart, or on the host."""
+    x, y, mask, table, tokens = saved_cases()
+    want = [f() for f in gradients(x, y, mask, ragged, table, tokens)]
+    apart = lambda t: torch.stack((t, t), -1)[..., 0]  # noqa: E731
+    for pack, unpack in ((lambda t: t.t().contiguous() if t.dim() == 2 else t, lambda t: t.t() if t.dim() == 2 else t),
+                         (apart, lambda t: t), (lambda t: t.cpu(), lambda t: t.cuda())):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            got = gradients(x, y, mask, ragged, table, tokens)
+        for f, w in zip(got, want):
+            assert torch.equal(f(), w)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_saved_tensors_that_come_back_as_others_are_refused(ragged):
+    """Of another type, another size or on another device: an error on the host, before anything is launched."""
+    x, y, mask, table, tokens = saved_cases()
+
+    def half(t):
+        return t.half() if t.is_floating_point() else t
+
+    def short(t):
+        return t[:-1]
+
+    def narrow(t):
+        return t.int() if t.dtype == torch.int64 else t
+
+    def host(t):
+        return t.cpu()
+
+    for unpack in (half, short, narrow, host):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            actions, embeddings = gradients(x, y, mask, ragged, table, tokens)
+        for f in (actions, embeddings) if unpack is not half else (actions,):
+            with pytest.raises((RuntimeError, ValueError), match="came back"):
+                f()
