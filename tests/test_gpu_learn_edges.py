@@ -14,6 +14,7 @@ pytestmark = pytest.mark.gpu
 
 from mymyr_b200 import _lib, learn  # noqa: E402
 from mymyr_b200.task import default_context  # noqa: E402
+from test_gpu_learn import DTYPES, HALF_ULP, TINY, near, plain  # noqa: E402
 
 INF = float("inf")
 EPS = 2.0 ** -24
@@ -123,6 +124,78 @@ def test_gradient_of_a_vector_without_rows(dtype, first):
         del held
         g, = torch.autograd.grad(got.entropy.sum() + got.logprob.sum(), leaf)
         assert g.shape == leaf.shape and (g == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", [[3, 0, 2, 2, 4] * 50, [2, 3] * 700, [0, 90, 1, 300] * 60, [1, 2] * 300 + [5000, 7]])
+def test_gradient_of_every_ragged_row(dtype, counts):
+    """All rows against 64 bits; the last counts put a long row into the layout of short ones."""
+    n, width = len(counts), max(counts)
+    count = torch.tensor(counts, device="cuda")
+    offsets = torch.cat((count.new_zeros(1), count.cumsum(0)))
+    total = int(offsets[-1])
+    flat = randn(total, seed=total, scale=2.0).to(dtype)
+    row = torch.repeat_interleave(torch.arange(n, device="cuda"), count)
+    place = torch.arange(total, device="cuda") - offsets[row]
+    x = torch.full((n, width), -INF, dtype=torch.float64, device="cuda")
+    x[row, place] = flat.double()
+    tokens = torch.where(count > 0, count // 2, -1)
+    gl, ge = randn(n, seed=1), randn(n, seed=2)
+    want = plain(x, tokens, None, 1.0, 6, gl, ge)
+    leaf = flat.clone().requires_grad_(True)
+    got = learn.logprobs(leaf, tokens, offsets=offsets, top=6)
+    assert torch.equal(got.top_tokens, want[3])
+    grad, = torch.autograd.grad((got.logprob, got.entropy), leaf, (gl, ge))
+    # the bounds of the dense form: the spread's roundings, a chain of sums (of up to 1,250 terms for four lanes)
+    tol = EPS * (4 * want[6] + 64 + (1250 if width == 5000 else 0))
+    size = gl.abs() + ge.abs() * (want[6] + want[1] + 1)
+    p, w = want[5][row, place], want[4][row, place]
+    bound = (tol * 4 * size)[row] * p + HALF_ULP[dtype] * w.abs() * 1.01 + 2 * TINY[dtype]
+    near(grad, w, bound + 4 * EPS * size[row] * (p + (w != 0)))
+
+
+@pytest.mark.parametrize("width", [30, 1000, 20000])
+def test_logprobs_of_rows_past_2_32_elements(width):
+    """Three rows, 2^31 + 8 elements apart: the third starts past 2^32 elements. So do its mask and its gradient."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB")
+    apart = 2 ** 31 + 8
+    big, wide = (torch.zeros(3, apart, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    allowed = torch.zeros(3, apart, dtype=torch.bool, device="cuda")
+    x, mask, grad = big[:, :width], allowed[:, :width], wide[:, :width]
+    x.copy_(randn(3, width, seed=width))
+    mask.copy_(randn(3, width, seed=width + 1) < 1)
+    y = mask.int().argmax(1)
+    got = learn.logprobs(x, y, mask=mask, top=3)
+    leaf = x.contiguous().requires_grad_(True)
+    want = learn.logprobs(leaf, y, mask=mask.contiguous(), top=3)
+    assert torch.equal(got.logprob, want.logprob.detach()) and torch.equal(got.entropy, want.entropy.detach())
+    assert torch.equal(got.top_tokens, want.top_tokens)
+    gl, ge, stats = randn(3, seed=1), randn(3, seed=2), torch.zeros(3, 4, device="cuda")
+    logprob, entropy = torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda")
+    L, h = _lib.lib(), default_context().handle
+    a = c_logprobs(x, y, mask=mask, mask_stride=apart, logprob=logprob, entropy=entropy, stats=stats)
+    assert L.b2_logprobs(h, C.byref(a), None) == 0, _lib.last_error()
+    assert L.b2_logprobs_backward(h, C.byref(a), gl.data_ptr(), ge.data_ptr(), grad.data_ptr(), apart,
+                                  None) == 0, _lib.last_error()
+    torch.cuda.synchronize()
+    each, = torch.autograd.grad((want.logprob, want.entropy), leaf, (gl, ge))
+    assert torch.equal(grad, each)
+    assert int(torch.count_nonzero(wide)) == int(torch.count_nonzero(each))
+
+
+def test_embedding_gradient_of_rows_past_2_32_elements():
+    free, _ = torch.cuda.mem_get_info()
+    if free < 20 << 30:
+        pytest.skip("needs 20 GB")
+    big = torch.zeros(3, 2 ** 31 + 8, dtype=torch.bfloat16, device="cuda")
+    g = big[:, :96]
+    g.copy_(randn(3, 96, seed=1))
+    w = torch.zeros(7, 96, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    tokens = torch.tensor([4, 2, 6], device="cuda")
+    grad, = torch.autograd.grad(learn.embedding(tokens, w), w, g)
+    assert torch.equal(grad[tokens], g) and (grad[[0, 1, 3, 5]] == 0).all()
 
 
 # ------------------------------------------------------------------------------------------------ AdamW
