@@ -194,11 +194,14 @@ __device__ __forceinline__ float above_least(float x)
 /// just advance between them.
 ///
 /// Bound by HBM in 32 bits: 28 bytes for an element (parameter, gradient and moments read, all but the gradient written),
-/// 174 M bf16 parameters with masters in 748 us (6.5 TB/s). With 8-bit moments it is 10 bytes and some 60 instructions,
-/// and these bound it: 329 M parameters in 682 us (4.9 TB/s). Five or three blocks an SM, fetching the next block ahead,
-/// taking elements in pairs or all arithmetic packed in pairs measured slower (registers, moves). One pass: everything of
-/// an element is in registers between its loads and its stores, the
-/// block's largest magnitudes come from the warp's 32-bit maximum reduction. Averages are separate multiplications and
+/// 174 M bf16 parameters with masters in 748 us (6.5 TB/s). With 8-bit moments it is 10 bytes and 66 instructions, and
+/// these bound it: 329 M parameters in 684 us (4.8 TB/s) at 1965 MHz, 742 in a long run at 1777 MHz under the power limit.
+/// Five or three blocks an SM, fetching the next block ahead, taking elements in pairs or all arithmetic packed in pairs
+/// measured slower (registers, moves). One pass: everything of an element is in registers between its loads and its
+/// stores, the block's largest magnitudes come from the warp's 32-bit maximum reduction.
+///
+/// The step's root and reciprocal are the fast ones (2 units in the last place of the step each); a stored root goes
+/// through one step of Heron's rule. Averages are separate multiplications and
 /// additions (not fused): the scales and codes then are those of the formula as written, on any machine.
 template<class P, class G, int BITS, bool MASTER, u32 N>
 __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant__ Table<N> t, const Moments s, const Hyper h,
@@ -395,8 +398,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_adamw(const __grid_constant_
                 }
             }
         };
-        // a tensor's last block, and tensors that start off a vector's boundary, go element by element (a body of their own:
-        // together with the others' it cost 10 %)
+        // a tensor's last block, and tensors that start off a vector's boundary, go element by element (170 M bf16 one
+        // element off: 778 us for 739 with 32-bit moments and masters, 456 for 367 with 8-bit ones), in a body of their own:
+        // together with the others' it cost 10 %
         if (aligned && n == kMoment)
             body.template operator()<true>();
         else

@@ -874,7 +874,8 @@ struct Gradient
         }
         else
         {
-            // a row's ends, rows that leave nothing, a gradient of another alignment; whole vectors still G at a time (a
+            // a row's ends, rows that leave nothing, a gradient of another alignment than its logits (8,192 rows of 50,257
+            // of 50,304 bf16: 1,020 us with the forward pass, 417 where they agree); whole vectors still G at a time (a
             // warp comes here with most of a short row; the larger blocks would lack the registers for more)
             constexpr int G = N == 32 ? U : 1;
 #pragma unroll 1
@@ -959,7 +960,9 @@ Rows rows_of(const b2_logprobs_args& a)
     return {a.logits, a.offsets, a.mask, a.row_stride, a.mask_stride, a.width, a.offsets_bits};
 }
 
-/// The mean length of a call's rows, by which they are laid out (ragged rows that are much longer are right, if slower).
+/// The mean length of a call's rows, by which they are laid out. Ragged rows that are much longer are right, if slower:
+/// 65,536 rows of 20 bf16 take 7.7 us forward and 63 with the gradient, with eight rows of 5,000 among them 38 and 193,
+/// with one of 100,000 639 and 3,600.
 u64 mean_length(const Rows& rows, u64 count) { return rows.offsets ? rows.width / count : rows.width; }
 
 /// How a call's rows are laid out.
@@ -1031,10 +1034,12 @@ void forward(const b2_ctx& ctx, const Forward& f, cudaStream_t st)
     while (cluster < 8 && f.count * cluster * 2 <= static_cast<u64>(ctx.sms) * 2 &&
            mean >= static_cast<u64>(cluster) * 2 * NW * 32 * kVec<T> * 2)
         cluster *= 2;
-    // a cluster's threads have few vectors each: all of them at once; blocks of 4 warps where rows are many and not long
-    // enough to make up for what a larger block waits for at their ends (16,384 rows of 15,000 bf16: 102 us, with 8 warps
-    // 134; 2,048 of 50,001 fp32 with 8 alternatives: 106 and 84), nor many alternatives to be looked for among few
-    // threads' logits (16,384 of 30,001 bf16 with 20: 344 and 314)
+    // A cluster's threads have few vectors each: all of them at once. Blocks of 4 warps where rows are many and not long
+    // enough to make up for what a larger block waits for at their ends (bf16, us with 4 and with 8 warps: 2,500 rows of
+    // 10,000 16.5 and 20.0, 16,384 of 15,000 102 and 134, 8,192 of 32,000 95 and 107, 6,000 of 50,257 111 and 120, 8,192 of
+    // 65,536 181 and 187; few or longer ones: 2,048 of 65,536 58 and 54, 3,000 of 32,000 43 and 44, 8,192 of 100,000 271
+    // and 277), nor many alternatives to be looked for among few threads' logits (2,048 of 50,001 fp32 with 8: 106 and 84,
+    // 16,384 of 30,001 bf16 with 20: 344 and 314; 8,192 of 24,000 bf16 with 5: 97 and 130)
     const bool few_warps = f.top <= 8 && mean <= (f.top ? 4096u : 8192u) * kVec<T> &&
                            f.count >= static_cast<u64>(ctx.sms) * (mean <= 2048 * kVec<T> ? 8 : 40);
     with_flags([&]<bool MASK, bool TOP>() {

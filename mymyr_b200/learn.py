@@ -72,7 +72,8 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, offset
 
     ``logits`` [..., V] with ``tokens`` [...]; or, with ``offsets`` [N + 1], a vector of all rows' logits with row r at
     offsets[r] .. offsets[r + 1] (the successors of ``rl.expand``) and ``tokens`` [N] counted within the row, as an
-    action of ``rl.BatchedEnv.step`` is. ``mask`` (bool, True: allowed) has the logits' shape or broadcasts to it.
+    action of ``rl.BatchedEnv.step`` is (for a gradient, offsets must not decrease: overlapping rows would overwrite one
+    another). ``mask`` (bool, True: allowed) has the logits' shape or broadcasts to it.
 
     A negative token is no token (log-probability 0, no gradient); a masked one, or any token of a row that leaves
     nothing, has -inf; one past the row gives NaN. Such a row has entropy 0, no alternatives and a zero gradient."""
