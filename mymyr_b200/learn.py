@@ -76,7 +76,8 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, offset
     another). ``mask`` (bool, True: allowed) has the logits' shape or broadcasts to it.
 
     A negative token is no token (log-probability 0, no gradient); a masked one, or any token of a row that leaves
-    nothing, has -inf; one past the row gives NaN. Such a row has entropy 0, no alternatives and a zero gradient."""
+    nothing, has -inf; one past the row gives NaN. A row that leaves nothing has entropy 0, no alternatives and a zero
+    gradient."""
     if stream is not None:
         with _on(stream, logits, tokens, offsets, mask):
             return LogProbs(*_learn.logprobs(logits, tokens, offsets, mask, temperature, top))
@@ -163,9 +164,12 @@ class AdamW:
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, bits: int = 32, master: bool = False, seed: int = 0):
         defaults = {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay}
+        if isinstance(params, torch.Tensor):  # its rows would be tensors without gradients
+            raise ValueError("AdamW: params must be a list of tensors or of groups")
         params = list(params)
         groups = params if params and isinstance(params[0], dict) else [{"params": params}]
-        self.param_groups = [defaults | g | {"params": list(g["params"])} for g in groups]
+        self.param_groups = [defaults | g | {"params": [p] if isinstance(p := g["params"], torch.Tensor) else list(p)}
+                             for g in groups]
         self.steps = 0
         self.param_steps = [[0] * len(g["params"]) for g in self.param_groups]
         self.seed = int(seed)

@@ -445,6 +445,19 @@ def test_adamw_object_with_gradients_now_and_then():
         late.load_state_dict(saved | {"param_steps": [[1, 2], [3]]})
 
 
+def test_adamw_takes_a_tensor_for_a_group_and_not_for_its_rows():
+    """A tensor is a list of its rows to Python, views that never have a gradient: nothing was updated."""
+    w, b = randn(6, 5, seed=1).requires_grad_(True), randn(5, seed=2).requires_grad_(True)
+    before = w.detach().clone(), b.detach().clone()
+    opt = learn.AdamW([{"params": w}, {"params": [b]}])
+    assert [len(g["params"]) for g in opt.param_groups] == [1, 1] and opt.param_groups[0]["params"][0] is w
+    w.grad, b.grad = torch.ones_like(w), torch.ones_like(b)
+    opt.step()
+    assert (w.detach() != before[0]).all() and (b.detach() != before[1]).all()
+    with pytest.raises(ValueError):
+        learn.AdamW(w)
+
+
 # ------------------------------------------------------------------------------------------------ saved tensors
 
 def gradients(x, y, mask, ragged, table, tokens):
