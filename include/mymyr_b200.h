@@ -487,7 +487,7 @@ b2_status b2_embedding_backward(b2_ctx* ctx, const b2_embedding_args* args, cons
 enum { B2_MOMENT_BLOCK = 256 };
 
 /* A tensor of an AdamW step: `elements` contiguous parameters and gradients, their moments from block `block` on
- * (element block * B2_MOMENT_BLOCK of the moment arrays; tensors do not share blocks). */
+ * (element block * B2_MOMENT_BLOCK of the moment arrays; tensors do not share blocks, nor parameters). */
 typedef struct b2_adamw_tensor {
     void* param;
     const void* grad;

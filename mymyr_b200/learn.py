@@ -135,7 +135,8 @@ def adamw_step(params, grads, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                exp_avg_scale: torch.Tensor | None = None, exp_avg_sq_scale: torch.Tensor | None = None,
                master: torch.Tensor | None = None, seed: int = 0, stream=None) -> None:
-    """One AdamW update of all ``params`` (contiguous, of any sizes) in place, with the moments of ``adamw_state``:
+    """One AdamW update of all ``params`` (contiguous, of any sizes, none overlapping) in place, with the moments of
+    ``adamw_state``:
 
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p = p (1 - lr weight_decay) - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)
@@ -170,6 +171,9 @@ class AdamW:
         groups = params if params and isinstance(params[0], dict) else [{"params": params}]
         self.param_groups = [defaults | g | {"params": [p] if isinstance(p := g["params"], torch.Tensor) else list(p)}
                              for g in groups]
+        every = [id(p) for g in self.param_groups for p in g["params"]]
+        if len(set(every)) < len(every):  # two threads would update the same numbers at once
+            raise ValueError("AdamW: a parameter is given twice")
         self.steps = 0
         self.param_steps = [[0] * len(g["params"]) for g in self.param_groups]
         self.seed = int(seed)

@@ -458,6 +458,14 @@ def test_adamw_takes_a_tensor_for_a_group_and_not_for_its_rows():
         learn.AdamW(w)
 
 
+def test_adamw_refuses_a_parameter_given_twice():
+    """A tied one, say: two entries of a launch would update it at once."""
+    w, b = randn(6, 5, seed=1).requires_grad_(True), randn(5, seed=2).requires_grad_(True)
+    for params in ([w, b, w], [{"params": [w]}, {"params": [b, w]}]):
+        with pytest.raises(ValueError, match="twice"):
+            learn.AdamW(params)
+
+
 # ------------------------------------------------------------------------------------------------ saved tensors
 
 def gradients(x, y, mask, ragged, table, tokens):
