@@ -4,7 +4,6 @@ ends of their range, steps that differ from parameter to parameter, arrays past 
 Tolerances come from the roundings a value goes through, EPS = 2^-24 each (32-bit arithmetic)."""
 
 import ctypes as C
-import math
 
 import pytest
 
